@@ -67,7 +67,11 @@ typedef enum sp24_dtype {
      (A __nv_fp8_e5m2, B __nv_fp8_e4m3). */
   SP24_E5M2_E4M3 = 3,
   SP24_E4M3_E5M2 = 4, /* no reference counterpart */
-  SP24_E5M2 = 5       /* A and B e5m2; no reference counterpart */
+  SP24_E5M2 = 5,      /* A and B e5m2; no reference counterpart */
+  /* Only where an entry point names them (the MLP-block operators below and
+     sp24_repack_meta); the plain GEMM refuses both. */
+  SP24_I8 = 6,        /* signed 8-bit integers */
+  SP24_F32 = 7        /* fp32 output of sp24_gemm_scaled */
 } sp24_dtype;
 
 typedef enum sp24_meta_format {
@@ -139,7 +143,8 @@ sp24_status sp24_prune_2of4(sp24_dtype dtype, const void* a, int m, int k, int64
                             void* a_pruned, int64_t ldp, sp24_stream_t stream);
 
 /* Repack reference-layout metadata into the tcgen05 image consumed by
-   sp24_gemm with SP24_META_TC.  Padding groups get the valid code 0x4. */
+   sp24_gemm with SP24_META_TC.  Padding groups get the valid code 0x4.
+   SP24_I8 has the image of the fp8 types. */
 sp24_status sp24_repack_meta(sp24_dtype dtype, const uint8_t* meta_ref, int m, int k,
                              uint8_t* meta_tc, sp24_stream_t stream);
 
@@ -244,6 +249,121 @@ typedef struct sp24_epilogue {
 /* sp24_gemm followed by the epilogue `e` (NULL = none), in one launch. */
 sp24_status sp24_gemm_fused(const sp24_gemm_desc* d, const sp24_epilogue* e,
                             sp24_stream_t stream);
+
+/* ------------------------------------------------------------------------
+   The MLP block (no counterpart in the reference, whose GEMM these surround).
+   Activations are token-major here: one row per token, its features
+   contiguous.  Zero tokens are a valid call that computes nothing (a weight
+   gradient over zero tokens is zero).  Row strides (ld*) count elements; 0
+   means the row's length.
+
+   Rows to 8 bits.  Each row y of the operator's result is stored as codes q
+   and one scale:
+     amax = max |y|,  scale = amax / Q,  q = round(y * Q / amax),  Q = 127 (SP24_I8)
+     or 448 (SP24_E4M3); int8 rounds half to even, e4m3 to nearest even.
+   A row of zeroes has scale 0 and codes 0.  A row that holds a NaN or an
+   infinity has scale NaN and codes 0, so everything computed from it is NaN.
+     sp24_rmsnorm_quant  s = x + residual (fp32; residual optional; its 16-bit
+                         rounding is written to residual_out when given, which
+                         may be the residual itself),
+                         y = s / sqrt(mean(s^2) + eps) * weight
+     sp24_swiglu_quant   y = silu(x) * up      (x: the gate projection)
+     sp24_quantize_rows  y = x                 (tokens, or the rows of a 16-bit
+                         A_c: the weights of sp24_gemm_scaled, one scale per
+                         output channel)
+   No alignment is required of any pointer or stride; rows whose pointers and
+   strides are 16-byte multiples take the vector path. */
+typedef struct sp24_rowquant_desc {
+  sp24_dtype dtype;            /* SP24_F16 or SP24_BF16: x, up, residual(_out), weight */
+  sp24_dtype qdtype;           /* SP24_I8 or SP24_E4M3 */
+  int rows, cols;              /* rows >= 0, cols >= 1 */
+  const void* x;               /* rows x cols */
+  int64_t ldx;
+  const void* up;              /* sp24_swiglu_quant only */
+  int64_t ld_up;
+  const void* residual;        /* sp24_rmsnorm_quant only, optional */
+  int64_t ld_residual;
+  void* residual_out;          /* optional; needs residual */
+  int64_t ld_residual_out;
+  const void* weight;          /* sp24_rmsnorm_quant only: cols values */
+  float eps;                   /* >= 0 */
+  void* q;                     /* rows x cols codes, one byte each */
+  int64_t ldq;
+  float* scale;                /* rows floats */
+} sp24_rowquant_desc;
+sp24_status sp24_rmsnorm_quant(const sp24_rowquant_desc* d, sp24_stream_t stream);
+sp24_status sp24_swiglu_quant(const sp24_rowquant_desc* d, sp24_stream_t stream);
+sp24_status sp24_quantize_rows(const sp24_rowquant_desc* d, sp24_stream_t stream);
+
+/* 8-bit product of n tokens with m x k 2:4 weights, a scale for each token and
+   each channel:
+     c[t][r] = scale_n[t] * scale_m[r] * sum_k x[t][k] W[r][k]  (+ bias[r])
+   SP24_I8 sums in 32-bit integers (exact; k <= 131072), SP24_E4M3 in fp32; the
+   scales and the bias are applied in fp32 and the result is rounded once to
+   cdtype.  k % 64 == 0.  a_c and x rows must start on 16-byte boundaries
+   (SP24_ERR_ALIGN); c has no alignment rule. */
+typedef struct sp24_scaled_desc {
+  sp24_dtype dtype;            /* SP24_I8 or SP24_E4M3: a_c and x */
+  sp24_dtype cdtype;           /* SP24_F16, SP24_BF16 or SP24_F32 */
+  int m, n, k;                 /* channels, tokens (>= 0), dense inner size */
+  const void* a_c;             /* compressed weights, m x k/2 */
+  int64_t lda_c;
+  const uint8_t* meta;         /* their tcgen05 image (sp24_repack_meta, dtype above) */
+  const void* x;               /* n x k */
+  int64_t ldx;
+  const float* scale_m;        /* m floats; NULL = 1 */
+  const float* scale_n;        /* n floats; NULL = 1 */
+  const float* bias;           /* m floats; NULL = none */
+  void* c;                     /* n x m */
+  int64_t ldc;
+  int* status_dev;             /* as in sp24_gemm_desc */
+} sp24_scaled_desc;
+sp24_status sp24_gemm_scaled(const sp24_scaled_desc* d, sp24_stream_t stream);
+
+/* Gated feed-forward block with dense 16-bit weights (a 2:4 model's weights
+   while they are trained), forward and backward:
+     g = x w_gate^T,  u = x w_up^T,  out = act(g) * u
+   and from d_out = dL/dout:
+     dg = d_out * u * act'(g),  du = d_out * act(g)
+     dx = dg w_gate + du w_up,  dw_gate = dg^T x,  dw_up = du^T x
+   Sums are fp32.  g and u are never rounded: the forward pass hands them to
+   the backward pass in fp32 through `saved`.  dg and du are rounded to dtype
+   (they are tensor-core operands); every output is rounded once.
+   x, w_gate and w_up rows must start on 16-byte boundaries (SP24_ERR_ALIGN);
+   so must saved and workspace.  out, d_out and the gradients have no alignment
+   rule. */
+typedef struct sp24_ffn_desc {
+  sp24_dtype dtype;            /* SP24_F16 or SP24_BF16: every tensor below */
+  int t, h, f;                 /* tokens (>= 0), input width, intermediate width */
+  sp24_activation act;         /* SP24_ACT_SILU, or SP24_ACT_NONE: g * u */
+  const void* x;               /* t x h */
+  int64_t ldx;
+  const void* w_gate;          /* f x h */
+  int64_t ld_gate;
+  const void* w_up;            /* f x h */
+  int64_t ld_up;
+  void* saved;                 /* forward: optional output; backward: its input */
+  size_t saved_bytes;          /* >= sp24_ffn_saved_bytes */
+  int* status_dev;             /* as in sp24_gemm_desc */
+} sp24_ffn_desc;
+typedef struct sp24_ffn_grads {
+  const void* d_out;           /* t x f */
+  int64_t ld_d_out;
+  void* dx;                    /* t x h; NULL = not wanted */
+  int64_t ld_dx;
+  void* dw_gate;               /* f x h, both or neither */
+  int64_t ld_dgate;
+  void* dw_up;
+  int64_t ld_dup;
+  void* workspace;             /* sp24_ffn_workspace_bytes */
+  size_t workspace_bytes;
+} sp24_ffn_grads;
+size_t sp24_ffn_saved_bytes(int t, int f);
+size_t sp24_ffn_workspace_bytes(int t, int f);
+sp24_status sp24_ffn_forward(const sp24_ffn_desc* d, void* out, int64_t ld_out,
+                             sp24_stream_t stream);
+sp24_status sp24_ffn_backward(const sp24_ffn_desc* d, const sp24_ffn_grads* g,
+                              sp24_stream_t stream);
 
 /* FP8 helpers.
    sp24_amax_f32: amax_dev[0] = max |x| over count floats (device).

@@ -34,10 +34,15 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall"]
 
-LIB_SOURCES = ["sp24_api.cu"]
 LIB_DEPS = ["sp24_api.cu", "sp24_gemm_kernel.cuh", "sp24_gemm2sm_kernel.cuh",
             "sp24_gemm_splitk_kernel.cuh", "sp24_prep.cuh",
-            "sp24_ptx.cuh"]
+            "sp24_ptx.cuh", "sp24_host.cuh"]
+# Translation units of the library and the files each one reads.
+LIB_UNITS = {
+    "sp24_api.cu": LIB_DEPS + [os.path.join("..", "dropin", "sp24_raw_kernel.cuh")],
+    "sp24_mlp.cu": ["sp24_mlp.cu", "sp24_host.cuh", "sp24_rows.cuh", "sp24_mlp_simple.cuh",
+                    "sp24_ptx.cuh"],
+}
 
 
 def _stale(target: str, deps) -> bool:
@@ -55,12 +60,28 @@ def _run(cmd, cwd=None) -> None:
 def build_lib(force: bool = False) -> str:
     os.makedirs(LIBDIR, exist_ok=True)
     out = os.path.join(LIBDIR, "libsp24.so")
-    deps = [os.path.join(CSRC, f) for f in LIB_DEPS] + [os.path.join(ROOT, "include", "sp24.h")]
-    if force or _stale(out, deps):
-        tmp = out + ".tmp"
-        _run([NVCC, *ARCH, *COMMON, "-shared", "-o", tmp,
-              *[os.path.join(CSRC, s) for s in LIB_SOURCES]])
-        os.replace(tmp, out)
+    objdir = os.path.join(HERE, "_build", "obj")
+    deps = {u: [os.path.join(CSRC, f) for f in fs] + [os.path.join(ROOT, "include", "sp24.h")]
+            for u, fs in LIB_UNITS.items()}
+    if not force and not _stale(out, [f for fs in deps.values() for f in fs]):
+        return out
+    os.makedirs(objdir, exist_ok=True)
+    objs, jobs = [], []
+    for unit, fs in deps.items():
+        obj = os.path.join(objdir, unit[:-3] + ".o")
+        objs.append(obj)
+        if force or _stale(obj, fs):
+            cmd = [NVCC, *ARCH, *COMMON, "-c", "-o", obj + ".tmp", os.path.join(CSRC, unit)]
+            print("+", " ".join(cmd), flush=True)
+            jobs.append((obj, cmd, subprocess.Popen(cmd)))
+    failed = [cmd for _, cmd, job in jobs if job.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    for obj, _, _ in jobs:
+        os.replace(obj + ".tmp", obj)
+    tmp = out + ".tmp"
+    _run([NVCC, *ARCH, "-shared", "-o", tmp, *objs])
+    os.replace(tmp, out)
     return out
 
 

@@ -20,13 +20,13 @@
 #include "sp24_gemm2sm_kernel.cuh"
 #include "sp24_gemm_kernel.cuh"
 #include "sp24_gemm_splitk_kernel.cuh"
+#include "sp24_host.cuh"
 #include "sp24_prep.cuh"
 #include "../dropin/sp24_raw_kernel.cuh"
 
-namespace {
+using namespace sp24host;
 
-constexpr int kMaxDevices = 64;
-constexpr unsigned long long kDefaultTimeoutNs = 1000000000ull;  // 1 s per bounded wait
+namespace {
 
 // Library-owned per-device status word used when the caller passes none.
 __device__ int g_sp24_status_word;
@@ -35,17 +35,6 @@ __device__ int g_sp24_status_word;
 // stand-in for the symbol: its device address comes from cudaGetSymbolAddress
 // (noalloc_scratch below), looked up once per device with that device current.
 static __device__ __align__(256) uint8_t g_sp24_noalloc_scratch[SP24_NOALLOC_SCRATCH_BYTES];
-
-#define SP24_CUDA_TRY(expr)                  \
-  do {                                       \
-    cudaError_t e__ = (expr);                \
-    if (e__ != cudaSuccess) {                \
-      (void)cudaGetLastError();              \
-      return SP24_ERR_CUDA;                  \
-    }                                        \
-  } while (0)
-
-inline cudaStream_t as_stream(sp24_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 
 inline bool is_fp8(int dt) { return dt >= SP24_E4M3 && dt <= SP24_E5M2; }
 inline int esize(sp24_dtype dt) { return is_fp8(dt) ? 1 : 2; }
@@ -58,14 +47,6 @@ inline uint32_t idesc_ab(int dt) {
   const uint32_t b = (dt == SP24_E4M3_E5M2 || dt == SP24_E5M2) ? 1u : 0u;
   return is_fp8(dt) ? (a << 7) | (b << 10) : 0u;
 }
-inline size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
-// 128-row blocks of the tcgen05 metadata image, padded to an even count so a
-// CTA pair's second half always has an atom to load.
-inline int meta_mblocks(int m) { return ((m + 127) / 128 + 1) / 2 * 2; }
-inline int meta_katoms(int k) { return (k + 127) / 128; }
-
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
 sp24_status get_encode_fn() {
@@ -100,16 +81,12 @@ sp24_status get_range_fn() {
   return g_range ? SP24_OK : SP24_ERR_CUDA;
 }
 
-struct DeviceInfo {
-  int sm_count = 0;
-  int* status_word = nullptr;
-  bool ok = false;
-};
-
 std::mutex g_dev_mu;
 DeviceInfo g_dev[kMaxDevices];
 
-sp24_status device_info(DeviceInfo** out) {
+}  // namespace
+
+sp24_status sp24host::device_info(DeviceInfo** out) {
   int dev = 0;
   SP24_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= kMaxDevices) return SP24_ERR_ARG;
@@ -129,9 +106,9 @@ sp24_status device_info(DeviceInfo** out) {
   return SP24_OK;
 }
 
-sp24_status encode_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner,
-                      uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer,
-                      CUtensorMapSwizzle sw) {
+sp24_status sp24host::encode_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base,
+                                uint64_t inner, uint64_t outer, uint64_t row_bytes,
+                                uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw) {
   sp24_status st = get_encode_fn();
   if (st != SP24_OK) return st;
   cuuint64_t dims[2] = {inner, outer};
@@ -143,6 +120,10 @@ sp24_status encode_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? SP24_OK : SP24_ERR_ALIGN;
 }
+
+std::mutex sp24host::g_attr_mu;
+
+namespace {
 
 CUtensorMapSwizzle swizzle_for_span(int span) {
   switch (span) {
@@ -227,28 +208,6 @@ Tuning tuning() {
   return g_tuning;
 }
 
-// Sets a kernel's function attributes (dynamic shared memory, and the
-// non-portable cluster size when asked) once per device.  `done` is the
-// calling launcher's own per-device flag array; the first calls on a device
-// from several host threads serialise on the mutex.
-std::mutex g_attr_mu;
-
-template <typename Kern>
-sp24_status ensure_kernel_attrs(Kern kern, std::atomic<bool> (&done)[kMaxDevices], int smem,
-                                bool nonportable_cluster = false) {
-  int dev = 0;
-  SP24_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= kMaxDevices) return SP24_ERR_ARG;
-  if (done[dev].load(std::memory_order_acquire)) return SP24_OK;
-  std::lock_guard<std::mutex> lk(g_attr_mu);
-  if (done[dev].load(std::memory_order_relaxed)) return SP24_OK;
-  SP24_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  if (nonportable_cluster)
-    SP24_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  done[dev].store(true, std::memory_order_release);
-  return SP24_OK;
-}
-
 // Everything a launch needs after validation / workspace staging.
 struct Prepared {
   sp24_dtype dt;
@@ -279,39 +238,6 @@ struct Prepared {
   int stall_producer;
   Tuning tune;          // the tuning switches in effect for this call
 };
-
-// GEMM launches carry programmatic stream serialization: the kernel may be
-// scheduled while the previous kernel of the stream finishes, runs its
-// prologue (barriers, TMEM allocation, tensor-map prefetch), and its TMA
-// producers wait for the previous grid (griddepcontrol.wait) before the
-// first load.  SP24_PDL=0 launches without the attribute.
-template <typename... KArgs, typename... Args>
-sp24_status launch_gemm_kernel(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem,
-                               cudaStream_t stream, unsigned cluster, bool pdl, Args&&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  unsigned na = 0;
-  if (cluster > 0) {   // run-time cluster shape; 0 = none (or the kernel's __cluster_dims__)
-    attr[na].id = cudaLaunchAttributeClusterDimension;
-    attr[na].val.clusterDim.x = cluster;
-    attr[na].val.clusterDim.y = 1;
-    attr[na].val.clusterDim.z = 1;
-    ++na;
-  }
-  if (pdl) {
-    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[na].val.programmaticStreamSerializationAllowed = 1;
-    ++na;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = na;
-  SP24_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...));
-  return SP24_OK;
-}
 
 template <int DT, int BN>
 sp24_status launch_gemm(const Prepared& p, const DeviceInfo& di, cudaStream_t stream) {
@@ -1607,15 +1533,16 @@ sp24_status sp24_prune_2of4(sp24_dtype dtype, const void* a, int m, int k, int64
 
 sp24_status sp24_repack_meta(sp24_dtype dtype, const uint8_t* meta_ref, int m, int k,
                              uint8_t* meta_tc, sp24_stream_t stream) {
-  if (!dtype_ok(dtype) || meta_ref == nullptr || meta_tc == nullptr) return SP24_ERR_ARG;
-  if (m <= 0 || k <= 0 || k % (is_fp8(dtype) ? 64 : 32) != 0) return SP24_ERR_SHAPE;
+  const bool is8 = is_fp8(dtype) || dtype == SP24_I8;
+  if ((!dtype_ok(dtype) && !is8) || meta_ref == nullptr || meta_tc == nullptr) return SP24_ERR_ARG;
+  if (m <= 0 || k <= 0 || k % (is8 ? 64 : 32) != 0) return SP24_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(meta_tc) & 3u) != 0) return SP24_ERR_ALIGN;
   const int mb = meta_mblocks(m);
   const int ka = meta_katoms(k);
   const long long total = static_cast<long long>(ka) * mb * 128 * 4;
   cudaStream_t s = as_stream(stream);
   sp24::repack_meta_kernel<<<grid_for(total, 256), 256, 0, s>>>(
-      meta_ref, m, k, is_fp8(dtype) ? 1 : 0, reinterpret_cast<uint32_t*>(meta_tc), mb, ka);
+      meta_ref, m, k, is8 ? 1 : 0, reinterpret_cast<uint32_t*>(meta_tc), mb, ka);
   SP24_CUDA_TRY(cudaGetLastError());
   return SP24_OK;
 }

@@ -1,0 +1,259 @@
+// sp24_mlp.cu — C ABI of the MLP-block operators declared in include/sp24.h:
+// argument checks and launches of the row kernels (sp24_rows.cuh), the 8-bit
+// scaled product and the gated feed-forward block.
+#include "sp24_host.cuh"
+#include "sp24_mlp_simple.cuh"
+#include "sp24_rows.cuh"
+
+using namespace sp24host;
+
+namespace {
+
+inline bool is_16bit(int dt) { return dt == SP24_F16 || dt == SP24_BF16; }
+
+// A row stride given as 0 means the row's length.
+inline int64_t stride_or(int64_t ld, int64_t len) { return ld ? ld : len; }
+
+// ------------------------------------------------------------------ rows to 8 bits
+sp24_status check_rows(const sp24_rowquant_desc* d, int mode, sp24::RowsParams* p) {
+  if (d == nullptr) return SP24_ERR_ARG;
+  if (!is_16bit(d->dtype) || (d->qdtype != SP24_I8 && d->qdtype != SP24_E4M3))
+    return SP24_ERR_ARG;
+  if (d->rows < 0 || d->cols <= 0) return SP24_ERR_SHAPE;
+  p->rows = d->rows;
+  p->cols = d->cols;
+  p->ldx = stride_or(d->ldx, d->cols);
+  p->ldq = stride_or(d->ldq, d->cols);
+  p->ld_up = stride_or(d->ld_up, d->cols);
+  p->ld_residual = stride_or(d->ld_residual, d->cols);
+  p->ld_residual_out = stride_or(d->ld_residual_out, d->cols);
+  if (p->ldx < d->cols || p->ldq < d->cols) return SP24_ERR_SHAPE;
+  if (mode == sp24::kRowsNorm) {
+    if (d->weight == nullptr || !(d->eps >= 0.0f)) return SP24_ERR_ARG;
+    if (d->residual_out != nullptr && d->residual == nullptr) return SP24_ERR_ARG;
+    if (p->ld_residual < d->cols || p->ld_residual_out < d->cols) return SP24_ERR_SHAPE;
+  } else if (d->residual != nullptr || d->residual_out != nullptr || d->weight != nullptr) {
+    return SP24_ERR_ARG;
+  }
+  if (mode == sp24::kRowsSwiglu) {
+    if (p->ld_up < d->cols) return SP24_ERR_SHAPE;
+  } else if (d->up != nullptr) {
+    return SP24_ERR_ARG;
+  }
+  if (d->rows > 0 && (d->x == nullptr || d->q == nullptr || d->scale == nullptr ||
+                      (mode == sp24::kRowsSwiglu && d->up == nullptr)))
+    return SP24_ERR_ARG;
+  p->x = d->x;
+  p->up = d->up;
+  p->residual = d->residual;
+  p->residual_out = d->residual_out;
+  p->weight = d->weight;
+  p->eps = d->eps;
+  p->q = static_cast<uint8_t*>(d->q);
+  p->scale = d->scale;
+  return SP24_OK;
+}
+
+template <int DT, int MODE, int I8>
+sp24_status launch_rows(const sp24::RowsParams& p, cudaStream_t s) {
+  sp24::rows_quant_kernel<DT, MODE, I8><<<static_cast<unsigned>(p.rows), 256, 0, s>>>(p);
+  SP24_CUDA_TRY(cudaGetLastError());
+  return SP24_OK;
+}
+
+template <int MODE>
+sp24_status rows_quant(const sp24_rowquant_desc* d, sp24_stream_t stream) {
+  sp24::RowsParams p{};
+  sp24_status st = check_rows(d, MODE, &p);
+  if (st != SP24_OK || d->rows == 0) return st;
+  DeviceInfo* di = nullptr;
+  st = device_info(&di);
+  if (st != SP24_OK) return st;
+  cudaStream_t s = as_stream(stream);
+  const bool i8 = d->qdtype == SP24_I8;
+  if (d->dtype == SP24_F16)
+    return i8 ? launch_rows<0, MODE, 1>(p, s) : launch_rows<0, MODE, 0>(p, s);
+  return i8 ? launch_rows<1, MODE, 1>(p, s) : launch_rows<1, MODE, 0>(p, s);
+}
+
+// ------------------------------------------------------------------ scaled product
+constexpr int kMaxScaledK = 131072;   // 2:4 int8 sums stay below 2^31 with room to spare
+
+sp24_status check_scaled(const sp24_scaled_desc* d) {
+  if (d == nullptr) return SP24_ERR_ARG;
+  if (d->dtype != SP24_I8 && d->dtype != SP24_E4M3) return SP24_ERR_ARG;
+  if (!is_16bit(d->cdtype) && d->cdtype != SP24_F32) return SP24_ERR_ARG;
+  if (d->m <= 0 || d->n < 0 || d->k <= 0 || d->k % 64 != 0) return SP24_ERR_SHAPE;
+  if (d->dtype == SP24_I8 && d->k > kMaxScaledK) return SP24_ERR_SHAPE;
+  const int64_t lda = stride_or(d->lda_c, d->k / 2), ldx = stride_or(d->ldx, d->k);
+  if (lda < d->k / 2 || ldx < d->k || stride_or(d->ldc, d->m) < d->m) return SP24_ERR_SHAPE;
+  if (d->a_c == nullptr || d->meta == nullptr) return SP24_ERR_ARG;
+  if (d->n > 0 && (d->x == nullptr || d->c == nullptr)) return SP24_ERR_ARG;
+  if (!aligned16(d->a_c) || !aligned16(d->meta) || !aligned16(d->x) || lda % 16 || ldx % 16)
+    return SP24_ERR_ALIGN;
+  return SP24_OK;
+}
+
+// ------------------------------------------------------------------ gated feed-forward
+// fp32 row stride of the saved planes, 16-bit row stride of the dg / du planes:
+// rows start on 32- and 16-byte boundaries.
+inline int64_t ffn_ld(int f) { return static_cast<int64_t>(round_up(static_cast<size_t>(f), 8)); }
+
+sp24_status check_ffn(const sp24_ffn_desc* d) {
+  if (d == nullptr) return SP24_ERR_ARG;
+  if (!is_16bit(d->dtype)) return SP24_ERR_ARG;
+  if (d->act != SP24_ACT_SILU && d->act != SP24_ACT_NONE) return SP24_ERR_ARG;
+  if (d->t < 0 || d->h <= 0 || d->f <= 0) return SP24_ERR_SHAPE;
+  const int64_t ldx = stride_or(d->ldx, d->h), ldg = stride_or(d->ld_gate, d->h),
+                ldu = stride_or(d->ld_up, d->h);
+  if (ldx < d->h || ldg < d->h || ldu < d->h) return SP24_ERR_SHAPE;
+  if (d->w_gate == nullptr || d->w_up == nullptr || (d->t > 0 && d->x == nullptr))
+    return SP24_ERR_ARG;
+  if (!aligned16(d->x) || !aligned16(d->w_gate) || !aligned16(d->w_up) || ldx % 8 || ldg % 8 ||
+      ldu % 8 || !aligned16(d->saved))
+    return SP24_ERR_ALIGN;
+  return SP24_OK;
+}
+
+template <int DT, int GATED>
+sp24_status launch_ffn_simple(const sp24::FfnSimpleParams& p, cudaStream_t s) {
+  const dim3 grid((p.nj + 15) / 16, (p.ni + 15) / 16);
+  sp24::ffn_simple_kernel<DT, GATED><<<grid, 256, 0, s>>>(p);
+  SP24_CUDA_TRY(cudaGetLastError());
+  return SP24_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+sp24_status sp24_rmsnorm_quant(const sp24_rowquant_desc* d, sp24_stream_t stream) {
+  return rows_quant<sp24::kRowsNorm>(d, stream);
+}
+
+sp24_status sp24_swiglu_quant(const sp24_rowquant_desc* d, sp24_stream_t stream) {
+  return rows_quant<sp24::kRowsSwiglu>(d, stream);
+}
+
+sp24_status sp24_quantize_rows(const sp24_rowquant_desc* d, sp24_stream_t stream) {
+  return rows_quant<sp24::kRowsPlain>(d, stream);
+}
+
+sp24_status sp24_gemm_scaled(const sp24_scaled_desc* d, sp24_stream_t stream) {
+  sp24_status st = check_scaled(d);
+  if (st != SP24_OK || d->n == 0) return st;
+  DeviceInfo* di = nullptr;
+  st = device_info(&di);
+  if (st != SP24_OK) return st;
+  sp24::ScaledParams p{};
+  p.m = d->m, p.n = d->n, p.k = d->k;
+  p.a_c = static_cast<const uint8_t*>(d->a_c);
+  p.lda_c = stride_or(d->lda_c, d->k / 2);
+  p.meta = d->meta;
+  p.meta_mblocks = meta_mblocks(d->m);
+  p.x = static_cast<const uint8_t*>(d->x);
+  p.ldx = stride_or(d->ldx, d->k);
+  p.scale_m = d->scale_m, p.scale_n = d->scale_n, p.bias = d->bias;
+  p.c = d->c;
+  p.ldc = stride_or(d->ldc, d->m);
+  p.cdtype = d->cdtype == SP24_F32 ? 2 : static_cast<int>(d->cdtype);
+  const dim3 grid((d->m + 15) / 16, (d->n + 15) / 16);
+  if (d->dtype == SP24_I8) sp24::scaled_simple_kernel<1><<<grid, 256, 0, as_stream(stream)>>>(p);
+  else sp24::scaled_simple_kernel<0><<<grid, 256, 0, as_stream(stream)>>>(p);
+  SP24_CUDA_TRY(cudaGetLastError());
+  return SP24_OK;
+}
+
+size_t sp24_ffn_saved_bytes(int t, int f) {
+  return t <= 0 || f <= 0 ? 0 : static_cast<size_t>(t) * 2 * ffn_ld(f) * sizeof(float);
+}
+
+size_t sp24_ffn_workspace_bytes(int t, int f) {
+  return t <= 0 || f <= 0 ? 0 : static_cast<size_t>(t) * 2 * ffn_ld(f) * 2;
+}
+
+sp24_status sp24_ffn_forward(const sp24_ffn_desc* d, void* out, int64_t ld_out,
+                             sp24_stream_t stream) {
+  sp24_status st = check_ffn(d);
+  if (st != SP24_OK) return st;
+  ld_out = stride_or(ld_out, d->f);
+  if (ld_out < d->f) return SP24_ERR_SHAPE;
+  if (d->t == 0) return SP24_OK;
+  if (out == nullptr) return SP24_ERR_ARG;
+  if (d->saved != nullptr && d->saved_bytes < sp24_ffn_saved_bytes(d->t, d->f))
+    return SP24_ERR_WORKSPACE;
+  DeviceInfo* di = nullptr;
+  st = device_info(&di);
+  if (st != SP24_OK) return st;
+  sp24::FfnSimpleParams p{};
+  p.ni = d->t, p.nj = d->f, p.nk = d->h, p.pairs = 1;
+  p.a[0] = d->x, p.b[0] = d->w_gate, p.b[1] = d->w_up;
+  p.a_i = stride_or(d->ldx, d->h), p.a_k = 1, p.b_k = 1, p.b_j = stride_or(d->ld_gate, d->h);
+  p.out = out, p.ldo = ld_out;
+  p.saved = static_cast<float*>(d->saved), p.ld_saved = ffn_ld(d->f);
+  p.silu = d->act == SP24_ACT_SILU;
+  return d->dtype == SP24_F16 ? launch_ffn_simple<0, 1>(p, as_stream(stream))
+                              : launch_ffn_simple<1, 1>(p, as_stream(stream));
+}
+
+sp24_status sp24_ffn_backward(const sp24_ffn_desc* d, const sp24_ffn_grads* g,
+                              sp24_stream_t stream) {
+  sp24_status st = check_ffn(d);
+  if (st != SP24_OK) return st;
+  if (g == nullptr) return SP24_ERR_ARG;
+  if ((g->dw_gate == nullptr) != (g->dw_up == nullptr)) return SP24_ERR_ARG;
+  const int64_t ldd = stride_or(g->ld_d_out, d->f), lddx = stride_or(g->ld_dx, d->h),
+                ldg = stride_or(g->ld_dgate, d->h), ldu = stride_or(g->ld_dup, d->h);
+  if (ldd < d->f || lddx < d->h || ldg < d->h || ldu < d->h) return SP24_ERR_SHAPE;
+  if (d->t > 0) {
+    if (g->d_out == nullptr || d->saved == nullptr) return SP24_ERR_ARG;
+    if (d->saved_bytes < sp24_ffn_saved_bytes(d->t, d->f) || g->workspace == nullptr ||
+        g->workspace_bytes < sp24_ffn_workspace_bytes(d->t, d->f))
+      return SP24_ERR_WORKSPACE;
+    if (!aligned16(g->workspace)) return SP24_ERR_ALIGN;
+  }
+  DeviceInfo* di = nullptr;
+  st = device_info(&di);
+  if (st != SP24_OK) return st;
+  cudaStream_t s = as_stream(stream);
+  if (d->t == 0) {   // sums over no token
+    if (g->dw_gate != nullptr) {
+      SP24_CUDA_TRY(cudaMemset2DAsync(g->dw_gate, ldg * 2, 0, d->h * 2, d->f, s));
+      SP24_CUDA_TRY(cudaMemset2DAsync(g->dw_up, ldu * 2, 0, d->h * 2, d->f, s));
+    }
+    return SP24_OK;
+  }
+  const bool f16 = d->dtype == SP24_F16;
+  const int64_t ldw = ffn_ld(d->f);
+  uint16_t* dg = static_cast<uint16_t*>(g->workspace);
+  uint16_t* du = dg + static_cast<size_t>(d->t) * ldw;
+  const dim3 eg((d->f + 255) / 256, d->t);
+  const int silu = d->act == SP24_ACT_SILU;
+  if (f16)
+    sp24::ffn_dgate_kernel<0><<<eg, 256, 0, s>>>(d->t, d->f, static_cast<const float*>(d->saved),
+                                                 ldw, g->d_out, ldd, silu, dg, ldw);
+  else
+    sp24::ffn_dgate_kernel<1><<<eg, 256, 0, s>>>(d->t, d->f, static_cast<const float*>(d->saved),
+                                                 ldw, g->d_out, ldd, silu, dg, ldw);
+  SP24_CUDA_TRY(cudaGetLastError());
+  sp24::FfnSimpleParams p{};
+  if (g->dx != nullptr) {
+    p.ni = d->t, p.nj = d->h, p.nk = d->f, p.pairs = 2;
+    p.a[0] = dg, p.a[1] = du, p.b[0] = d->w_gate, p.b[1] = d->w_up;
+    p.a_i = ldw, p.a_k = 1, p.b_k = stride_or(d->ld_gate, d->h), p.b_j = 1;
+    p.out = g->dx, p.ldo = lddx;
+    st = f16 ? launch_ffn_simple<0, 0>(p, s) : launch_ffn_simple<1, 0>(p, s);
+    if (st != SP24_OK) return st;
+  }
+  for (int w = 0; w < 2 && g->dw_gate != nullptr; ++w) {
+    p.ni = d->f, p.nj = d->h, p.nk = d->t, p.pairs = 1;
+    p.a[0] = w ? du : dg, p.b[0] = d->x;
+    p.a_i = 1, p.a_k = ldw, p.b_k = stride_or(d->ldx, d->h), p.b_j = 1;
+    p.out = w ? g->dw_up : g->dw_gate, p.ldo = w ? ldu : ldg;
+    st = f16 ? launch_ffn_simple<0, 0>(p, s) : launch_ffn_simple<1, 0>(p, s);
+    if (st != SP24_OK) return st;
+  }
+  return SP24_OK;
+}
+
+}  // extern "C"

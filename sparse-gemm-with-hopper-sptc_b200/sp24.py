@@ -24,6 +24,8 @@ PEAK_LIB_PATH = os.path.join(HERE, "lib", "libsp24_peak.so")
 F16, BF16, E4M3 = 0, 1, 2
 # Mixed fp8: A's format first, B's second (kind::f8f6f4 formats may differ).
 E5M2_E4M3, E4M3_E5M2, E5M2 = 3, 4, 5
+# Rows and products of the MLP block: 8-bit integers, fp32 output.
+I8, F32 = 6, 7
 META_REF, META_TC, META_K16 = 0, 1, 2
 
 STATUS = {
@@ -42,6 +44,8 @@ EXPORTS = [
     "sp24_gemm_allgather", "sp24_ipc_get_handle", "sp24_ipc_open_handle", "sp24_ipc_close",
     "sp24_set_launch_hints", "sp24_get_launch_hints", "sp24_reload_tuning",
     "sp24_gemm_multi", "sp24_replicate", "sp24_gemm_multi_workspace_bytes",
+    "sp24_rmsnorm_quant", "sp24_swiglu_quant", "sp24_quantize_rows", "sp24_gemm_scaled",
+    "sp24_ffn_forward", "sp24_ffn_backward", "sp24_ffn_saved_bytes", "sp24_ffn_workspace_bytes",
 ]
 MAX_PEERS = 7
 HINT_NONE, HINT_STATIC_WEIGHTS = 0, 1
@@ -91,6 +95,44 @@ class MultiDesc(Structure):
         ("meta", c_void_p * MAX_GPUS), ("b", c_void_p * MAX_GPUS), ("b_layout", c_int),
         ("c_f32", c_void_p * MAX_GPUS), ("c_bf16", c_void_p * MAX_GPUS), ("c_layout", c_int),
         ("workspace", c_void_p * MAX_GPUS), ("workspace_bytes", c_size_t),
+    ]
+
+
+class RowQuantDesc(Structure):
+    _fields_ = [
+        ("dtype", c_int), ("qdtype", c_int), ("rows", c_int), ("cols", c_int),
+        ("x", c_void_p), ("ldx", c_int64), ("up", c_void_p), ("ld_up", c_int64),
+        ("residual", c_void_p), ("ld_residual", c_int64),
+        ("residual_out", c_void_p), ("ld_residual_out", c_int64),
+        ("weight", c_void_p), ("eps", c_float), ("q", c_void_p), ("ldq", c_int64),
+        ("scale", c_void_p),
+    ]
+
+
+class ScaledDesc(Structure):
+    _fields_ = [
+        ("dtype", c_int), ("cdtype", c_int), ("m", c_int), ("n", c_int), ("k", c_int),
+        ("a_c", c_void_p), ("lda_c", c_int64), ("meta", c_void_p),
+        ("x", c_void_p), ("ldx", c_int64),
+        ("scale_m", c_void_p), ("scale_n", c_void_p), ("bias", c_void_p),
+        ("c", c_void_p), ("ldc", c_int64), ("status_dev", c_void_p),
+    ]
+
+
+class FfnDesc(Structure):
+    _fields_ = [
+        ("dtype", c_int), ("t", c_int), ("h", c_int), ("f", c_int), ("act", c_int),
+        ("x", c_void_p), ("ldx", c_int64), ("w_gate", c_void_p), ("ld_gate", c_int64),
+        ("w_up", c_void_p), ("ld_up", c_int64),
+        ("saved", c_void_p), ("saved_bytes", c_size_t), ("status_dev", c_void_p),
+    ]
+
+
+class FfnGrads(Structure):
+    _fields_ = [
+        ("d_out", c_void_p), ("ld_d_out", c_int64), ("dx", c_void_p), ("ld_dx", c_int64),
+        ("dw_gate", c_void_p), ("ld_dgate", c_int64), ("dw_up", c_void_p), ("ld_dup", c_int64),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
     ]
 
 
@@ -148,7 +190,17 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
                                        POINTER(c_int)]
     lib.sp24_unshard_columns_f32.argtypes = [c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                              c_void_p]
-    for name in ("sp24_gemm", "sp24_gemm_noalloc", "sp24_gemm_fused", "sp24_gemm_allgather",
+    for name in ("sp24_rmsnorm_quant", "sp24_swiglu_quant", "sp24_quantize_rows"):
+        getattr(lib, name).argtypes = [POINTER(RowQuantDesc), c_void_p]
+        getattr(lib, name).restype = c_int
+    lib.sp24_gemm_scaled.argtypes = [POINTER(ScaledDesc), c_void_p]
+    lib.sp24_ffn_forward.argtypes = [POINTER(FfnDesc), c_void_p, c_int64, c_void_p]
+    lib.sp24_ffn_backward.argtypes = [POINTER(FfnDesc), POINTER(FfnGrads), c_void_p]
+    for name in ("sp24_ffn_saved_bytes", "sp24_ffn_workspace_bytes"):
+        getattr(lib, name).argtypes = [c_int, c_int]
+        getattr(lib, name).restype = c_size_t
+    for name in ("sp24_gemm_scaled", "sp24_ffn_forward", "sp24_ffn_backward",
+                 "sp24_gemm", "sp24_gemm_noalloc", "sp24_gemm_fused", "sp24_gemm_allgather",
                  "sp24_gemm_multi", "sp24_replicate",
                  "sp24_ipc_get_handle", "sp24_ipc_open_handle", "sp24_ipc_close",
                  "sp24_selftest_timeout",
@@ -322,6 +374,237 @@ def gemm_fused(a_c, meta, b, m, n, k, *, bias=None, act=ACT_NONE, a_c_up=None, m
     _check(lib.sp24_gemm_fused(ctypes.byref(d), ctypes.byref(e), _stream(stream)),
            "sp24_gemm_fused")
     return c_f32, c_bf16
+
+
+# ------------------------------------------------------------------ the MLP block
+# Activations are token-major: one row per token, its features contiguous.
+
+def _rows2d(t, what, cols=None, rows=None):
+    """A CUDA matrix whose rows are contiguous (any row stride)."""
+    if not t.is_cuda or t.dim() != 2:
+        raise ValueError(f"{what}: a 2-D CUDA tensor is wanted")
+    if (cols is not None and t.shape[1] != cols) or (rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected "
+                         f"({'any' if rows is None else rows}, {'any' if cols is None else cols})")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1] or (t.shape[1] > 1 and t.stride(1) != 1):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t):
+    """Row stride in elements; a single row's stride says nothing."""
+    return t.stride(0) if t.shape[0] > 1 else 0
+
+
+def _tma_rows(t, what, cols=None, rows=None):
+    """_rows2d whose rows also start on 16-byte boundaries (TMA operands):
+    others are copied into padded rows first."""
+    t = _rows2d(t, what, cols, rows)
+    unit = 16 // t.element_size()
+    if t.data_ptr() % 16 == 0 and (t.shape[0] == 1 and t.shape[1] % unit == 0
+                                   or t.shape[0] > 1 and t.stride(0) % unit == 0):
+        return t
+    ld = (t.shape[1] + unit - 1) // unit * unit
+    padded = t.new_empty((t.shape[0], ld))[:, :t.shape[1]]
+    padded.copy_(t)
+    return padded
+
+
+def _tma_ld(t):
+    unit = 16 // t.element_size()
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + unit - 1) // unit * unit
+
+
+def _same_device(*ts):
+    devs = {t.device for t in ts if t is not None}
+    if len(devs) != 1:
+        raise ValueError(f"tensors on several devices: {sorted(map(str, devs))}")
+    return devs.pop()
+
+
+class _On:
+    """Work of one call: its device current and its stream torch's current one,
+    so that copies and outputs made on the way are ordered with the kernels."""
+
+    def __init__(self, device, stream):
+        import torch
+        self.dev = torch.cuda.device(device)
+        self.ctx = torch.cuda.stream(stream) if stream is not None else None
+        self.device = device
+
+    def __enter__(self):
+        import torch
+        self.dev.__enter__()
+        if self.ctx is not None:
+            self.ctx.__enter__()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+        self.dev.__exit__(*exc)
+
+
+def _quant_dtype(qdtype):
+    import torch
+    if qdtype == I8:
+        return torch.int8
+    if qdtype == E4M3:
+        return torch.float8_e4m3fn
+    raise ValueError(f"qdtype {qdtype}: I8 or E4M3")
+
+
+def _rows_quant(entry, x, qdtype, stream, up=None, weight=None, residual=None, eps=0.0):
+    import torch
+    lib = load()
+    code_dtype = _quant_dtype(qdtype)
+    for t in (up, weight, residual):
+        if t is not None and t.dtype != x.dtype:
+            raise ValueError(f"{entry}: {t.dtype} beside {x.dtype}")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{entry}: float16 or bfloat16 rows, not {x.dtype}")
+    with _On(_same_device(x, up, weight, residual), stream) as s:
+        x = _rows2d(x, "x")
+        rows, cols = x.shape
+        d = RowQuantDesc()
+        d.dtype, d.qdtype, d.rows, d.cols = dtype_code(x.dtype), qdtype, rows, cols
+        d.x, d.ldx = _ptr(x), _ld(x)
+        if up is not None:
+            up = _rows2d(up, "up", cols, rows)
+            d.up, d.ld_up = _ptr(up), _ld(up)
+        total = None
+        if weight is not None:
+            if weight.shape != (cols,):
+                raise ValueError(f"weight: shape {tuple(weight.shape)}, expected ({cols},)")
+            weight = weight.contiguous()
+            d.weight, d.eps = _ptr(weight), eps
+        if residual is not None:
+            residual = _rows2d(residual, "residual", cols, rows)
+            total = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+            d.residual, d.ld_residual, d.residual_out = _ptr(residual), _ld(residual), _ptr(total)
+        q = torch.empty((rows, cols), dtype=code_dtype, device=x.device)
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+        d.q, d.scale = _ptr(q), _ptr(scale)
+        _check(getattr(lib, entry)(ctypes.byref(d), s), entry)
+    return (q, scale) if residual is None else (q, scale, total)
+
+
+def rmsnorm_quant(x, weight, residual=None, *, eps=1e-6, qdtype=I8, stream=None):
+    """sp24_rmsnorm_quant: 8-bit rows of rmsnorm(x [+ residual]) * weight.
+    Returns (q, scale), or (q, scale, x + residual) when a residual is given;
+    a row's values are q * scale."""
+    return _rows_quant("sp24_rmsnorm_quant", x, qdtype, stream, weight=weight, residual=residual,
+                       eps=eps)
+
+
+def swiglu_quant(gate, up, *, qdtype=I8, stream=None):
+    """sp24_swiglu_quant: 8-bit rows of silu(gate) * up -> (q, scale)."""
+    return _rows_quant("sp24_swiglu_quant", gate, qdtype, stream, up=up)
+
+
+def quantize_rows(x, *, qdtype=I8, stream=None):
+    """sp24_quantize_rows: 8-bit rows of x -> (q, scale).  Applied to a 16-bit
+    A_c it gives the 8-bit weights of gemm_scaled and their channel scales."""
+    return _rows_quant("sp24_quantize_rows", x, qdtype, stream)
+
+
+def gemm_scaled(a_c, meta_tc, x, scale_w=None, scale_x=None, *, bias=None, out_dtype=None,
+                stream=None):
+    """sp24_gemm_scaled: tokens x [n, k] (int8 or e4m3) times the 2:4 weights
+    (a_c [m, k/2] of the same type, tcgen05 metadata image) with a scale for
+    each channel (scale_w [m]) and each token (scale_x [n]) -> [n, m] of
+    out_dtype (bfloat16, float16 or float32; default bfloat16)."""
+    import torch
+    lib = load()
+    out_dtype = out_dtype or torch.bfloat16
+    codes = {torch.int8: I8, torch.float8_e4m3fn: E4M3}
+    outs = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
+    if x.dtype not in codes or a_c.dtype != x.dtype:
+        raise ValueError(f"gemm_scaled: {x.dtype} tokens and {a_c.dtype} weights; both int8 or "
+                         "both float8_e4m3fn are wanted")
+    if out_dtype not in outs:
+        raise ValueError(f"gemm_scaled: out_dtype {out_dtype}")
+    with _On(_same_device(a_c, meta_tc, x, scale_w, scale_x, bias), stream) as s:
+        a_c = _tma_rows(a_c, "a_c")
+        m, k = a_c.shape[0], 2 * a_c.shape[1]
+        x = _tma_rows(x, "x", k)
+        n = x.shape[0]
+        if meta_tc.numel() * meta_tc.element_size() != meta_tc_bytes(m, k):
+            raise ValueError(f"meta_tc: {meta_tc.numel()} bytes, {meta_tc_bytes(m, k)} expected")
+        keep = []
+        for t, size, what in ((scale_w, m, "scale_w"), (scale_x, n, "scale_x"), (bias, m, "bias")):
+            if t is not None and (t.dtype != torch.float32 or t.numel() != size):
+                raise ValueError(f"{what}: {size} float32 values are wanted")
+            keep.append(t if t is None else t.contiguous())
+        c = torch.empty((n, m), dtype=out_dtype, device=x.device)
+        d = ScaledDesc()
+        d.dtype, d.cdtype, d.m, d.n, d.k = codes[x.dtype], outs[out_dtype], m, n, k
+        d.a_c, d.lda_c, d.meta = _ptr(a_c), _tma_ld(a_c), _ptr(meta_tc)
+        d.x, d.ldx = _ptr(x), _tma_ld(x)
+        d.scale_m, d.scale_n, d.bias = (_ptr(t) for t in keep)
+        d.c = _ptr(c)
+        _check(lib.sp24_gemm_scaled(ctypes.byref(d), s), "sp24_gemm_scaled")
+    return c
+
+
+def _ffn_desc(x, w_gate, w_up, act):
+    import torch
+    if x.dtype not in (torch.float16, torch.bfloat16) or {w_gate.dtype, w_up.dtype} != {x.dtype}:
+        raise ValueError(f"ffn_gated: {x.dtype}, {w_gate.dtype}, {w_up.dtype}; one of float16 and "
+                         "bfloat16 for all is wanted")
+    x = _tma_rows(x, "x")
+    w_gate = _tma_rows(w_gate, "w_gate", x.shape[1])
+    w_up = _tma_rows(w_up, "w_up", x.shape[1], w_gate.shape[0])
+    d = FfnDesc()
+    d.dtype, d.act = dtype_code(x.dtype), act
+    d.t, d.h, d.f = x.shape[0], x.shape[1], w_gate.shape[0]
+    d.x, d.ldx = _ptr(x), _tma_ld(x)
+    d.w_gate, d.ld_gate, d.w_up, d.ld_up = _ptr(w_gate), _tma_ld(w_gate), _ptr(w_up), _tma_ld(w_up)
+    return d, (x, w_gate, w_up)
+
+
+def ffn_gated(x, w_gate, w_up, *, act=ACT_SILU, save=False, stream=None):
+    """sp24_ffn_forward: act(x w_gate^T) * (x w_up^T) -> [t, f]; with save=True
+    also the opaque buffer that ffn_gated_backward takes."""
+    import torch
+    lib = load()
+    with _On(_same_device(x, w_gate, w_up), stream) as s:
+        d, keep = _ffn_desc(x, w_gate, w_up, act)
+        out = torch.empty((d.t, d.f), dtype=x.dtype, device=x.device)
+        saved = None
+        if save:
+            saved = torch.empty(lib.sp24_ffn_saved_bytes(d.t, d.f), dtype=torch.uint8,
+                                device=x.device)
+            d.saved, d.saved_bytes = _ptr(saved), saved.numel()
+        _check(lib.sp24_ffn_forward(ctypes.byref(d), _ptr(out), 0, s), "sp24_ffn_forward")
+        del keep
+    return (out, saved) if save else out
+
+
+def ffn_gated_backward(d_out, x, w_gate, w_up, saved, *, act=ACT_SILU, need_dx=True,
+                       need_dw=True, stream=None):
+    """sp24_ffn_backward: (dx, dw_gate, dw_up) from dL/dout and what
+    ffn_gated(save=True) kept (None for gradients that are not wanted)."""
+    import torch
+    lib = load()
+    if d_out.dtype != x.dtype:
+        raise ValueError(f"ffn_gated_backward: {d_out.dtype} beside {x.dtype}")
+    with _On(_same_device(d_out, x, w_gate, w_up, saved), stream) as s:
+        d, keep = _ffn_desc(x, w_gate, w_up, act)
+        d_out = _rows2d(d_out, "d_out", d.f, d.t)
+        d.saved, d.saved_bytes = _ptr(saved), saved.numel()
+        new = lambda *shape: torch.empty(shape, dtype=x.dtype, device=x.device)  # noqa: E731
+        dx = new(d.t, d.h) if need_dx else None
+        dw_gate, dw_up = (new(d.f, d.h), new(d.f, d.h)) if need_dw else (None, None)
+        ws = torch.empty(lib.sp24_ffn_workspace_bytes(d.t, d.f), dtype=torch.uint8,
+                         device=x.device)
+        g = FfnGrads()
+        g.d_out, g.ld_d_out = _ptr(d_out), _ld(d_out)
+        g.dx, g.dw_gate, g.dw_up = _ptr(dx), _ptr(dw_gate), _ptr(dw_up)
+        g.workspace, g.workspace_bytes = _ptr(ws), ws.numel()
+        _check(lib.sp24_ffn_backward(ctypes.byref(d), ctypes.byref(g), s), "sp24_ffn_backward")
+        del keep
+    return dx, dw_gate, dw_up
 
 
 def ipc_handle(t):

@@ -1,0 +1,152 @@
+"""The MLP-block operators without a GPU: what their descriptors refuse before
+any CUDA call, their buffer sizes, and what the torch-facing shim refuses."""
+import ctypes
+
+import pytest
+import torch
+
+import sp24
+
+P = 0x10000   # a non-null, 16-byte aligned "pointer"; refused calls never read it
+
+
+def _fill(d, base, kw):
+    for k, v in {**base, **kw}.items():
+        setattr(d, k, v)
+    return ctypes.byref(d)
+
+
+ROWS = dict(dtype=1, qdtype=sp24.I8, rows=4, cols=64, x=P, q=P, scale=P)
+
+
+@pytest.mark.parametrize("entry,kw,code", [
+    ("sp24_quantize_rows", dict(dtype=2), 8),                    # 16-bit rows only
+    ("sp24_quantize_rows", dict(dtype=sp24.I8), 8),
+    ("sp24_quantize_rows", dict(qdtype=5), 8),                   # e5m2 codes are not offered
+    ("sp24_quantize_rows", dict(qdtype=1), 8),
+    ("sp24_quantize_rows", dict(cols=0), 1),
+    ("sp24_quantize_rows", dict(rows=-1), 1),
+    ("sp24_quantize_rows", dict(ldx=63), 1),
+    ("sp24_quantize_rows", dict(ldq=8), 1),
+    ("sp24_quantize_rows", dict(x=None), 8),
+    ("sp24_quantize_rows", dict(q=None), 8),
+    ("sp24_quantize_rows", dict(scale=None), 8),
+    ("sp24_quantize_rows", dict(weight=P), 8),                   # another operator's fields
+    ("sp24_quantize_rows", dict(up=P), 8),
+    ("sp24_quantize_rows", dict(residual=P), 8),
+    ("sp24_swiglu_quant", dict(), 8),                            # no up
+    ("sp24_swiglu_quant", dict(up=P, ld_up=32), 1),
+    ("sp24_swiglu_quant", dict(up=P, residual_out=P), 8),
+    ("sp24_rmsnorm_quant", dict(), 8),                           # no weight
+    ("sp24_rmsnorm_quant", dict(weight=P, eps=-1.0), 8),
+    ("sp24_rmsnorm_quant", dict(weight=P, eps=float("nan")), 8),
+    ("sp24_rmsnorm_quant", dict(weight=P, up=P), 8),
+    ("sp24_rmsnorm_quant", dict(weight=P, residual_out=P), 8),   # a sum of nothing
+    ("sp24_rmsnorm_quant", dict(weight=P, residual=P, ld_residual=8), 1),
+    ("sp24_quantize_rows", dict(rows=0, x=None, q=None, scale=None), 0),
+])
+def test_rows_refusals(entry, kw, code):
+    lib = sp24.load()
+    assert getattr(lib, entry)(_fill(sp24.RowQuantDesc(), ROWS, kw), None) == code
+    assert getattr(lib, entry)(None, None) == 8
+
+
+SCALED = dict(dtype=sp24.I8, cdtype=1, m=128, n=16, k=128, a_c=P, meta=P, x=P, c=P)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=1), 8), (dict(dtype=5), 8), (dict(dtype=7), 8),
+    (dict(cdtype=2), 8), (dict(cdtype=sp24.I8), 8),
+    (dict(m=0), 1), (dict(n=-1), 1), (dict(k=0), 1), (dict(k=96), 1),
+    (dict(k=131136), 1),                      # int8 sums could leave 32 bits
+    (dict(lda_c=32), 1), (dict(ldx=64), 1), (dict(ldc=64), 1),
+    (dict(a_c=None), 8), (dict(meta=None), 8), (dict(x=None), 8), (dict(c=None), 8),
+    (dict(a_c=P + 8), 2), (dict(x=P + 4), 2), (dict(meta=P + 2), 2),
+    (dict(lda_c=72), 2), (dict(ldx=136), 2),
+    (dict(n=0, x=None, c=None), 0),
+])
+def test_scaled_refusals(kw, code):
+    lib = sp24.load()
+    assert lib.sp24_gemm_scaled(_fill(sp24.ScaledDesc(), SCALED, kw), None) == code
+    assert lib.sp24_gemm_scaled(None, None) == 8
+
+
+FFN = dict(dtype=1, t=4, h=64, f=96, act=1, x=P, w_gate=P, w_up=P)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=2), 8), (dict(dtype=7), 8), (dict(act=2), 8),
+    (dict(t=-1), 1), (dict(h=0), 1), (dict(f=0), 1),
+    (dict(ldx=63), 1), (dict(ld_gate=56), 1), (dict(ld_up=8), 1),
+    (dict(x=None), 8), (dict(w_gate=None), 8), (dict(w_up=None), 8),
+    (dict(x=P + 2), 2), (dict(w_up=P + 8), 2), (dict(ldx=68), 2), (dict(h=63), 2),
+    (dict(saved=P, saved_bytes=4 * 2 * 96 * 4 - 1), 9),
+    (dict(t=0, x=None), 0),
+])
+def test_ffn_forward_refusals(kw, code):
+    lib = sp24.load()
+    assert lib.sp24_ffn_forward(_fill(sp24.FfnDesc(), FFN, kw), P, 0, None) == code
+    assert lib.sp24_ffn_forward(None, P, 0, None) == 8
+    assert lib.sp24_ffn_forward(_fill(sp24.FfnDesc(), FFN, {}), None, 0, None) == 8
+    assert lib.sp24_ffn_forward(_fill(sp24.FfnDesc(), FFN, {}), P, 95, None) == 1
+
+
+@pytest.mark.parametrize("kw,gkw,code", [
+    ({}, dict(dw_up=None), 8),                # one weight gradient without the other
+    ({}, dict(d_out=None), 8),
+    (dict(saved=None), {}, 8),
+    (dict(saved_bytes=100), {}, 9),
+    ({}, dict(workspace=None), 9),
+    ({}, dict(workspace_bytes=100), 9),
+    ({}, dict(workspace=P + 4), 2),
+    ({}, dict(ld_d_out=95), 1),
+    ({}, dict(ld_dx=63), 1),
+    ({}, dict(ld_dgate=63), 1),
+    (dict(act=3), {}, 8),
+])
+def test_ffn_backward_refusals(kw, gkw, code):
+    lib = sp24.load()
+    need = lib.sp24_ffn_workspace_bytes(4, 96)
+    base = dict(FFN, saved=P, saved_bytes=lib.sp24_ffn_saved_bytes(4, 96))
+    grads = dict(d_out=P, dx=P, dw_gate=P, dw_up=P, workspace=P, workspace_bytes=need)
+    d = _fill(sp24.FfnDesc(), base, kw)
+    assert lib.sp24_ffn_backward(d, _fill(sp24.FfnGrads(), grads, gkw), None) == code
+    assert lib.sp24_ffn_backward(d, None, None) == 8
+
+
+def test_ffn_buffer_sizes():
+    lib = sp24.load()
+    assert lib.sp24_ffn_saved_bytes(3, 10) == 3 * 2 * 16 * 4     # rows of 16 floats
+    assert lib.sp24_ffn_workspace_bytes(3, 10) == 3 * 2 * 16 * 2
+    assert lib.sp24_ffn_saved_bytes(0, 10) == lib.sp24_ffn_workspace_bytes(5, 0) == 0
+    assert lib.sp24_ffn_saved_bytes(70000, 14336) == 70000 * 2 * 14336 * 4   # past 32 bits
+
+
+def test_plain_gemm_still_refuses_the_new_types():
+    lib = sp24.load()
+    d = sp24.GemmDesc()
+    d.m = d.n = d.k = 128
+    d.a_c = d.meta = d.b = d.c_f32 = P
+    d.meta_format = sp24.META_TC
+    for dtype in (sp24.I8, sp24.F32):
+        d.dtype = dtype
+        assert lib.sp24_gemm(ctypes.byref(d), None) == 8
+        assert lib.sp24_prune_2of4(dtype, P, 8, 8, 0, P, 0, None) == 8
+    assert lib.sp24_repack_meta(sp24.F32, P, 64, 64, P, None) == 8
+    assert lib.sp24_repack_meta(sp24.I8, P, 64, 32, P, None) == 1    # k % 64 as for fp8
+
+
+def test_shim_refusals():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        sp24.quantize_rows(x, qdtype=sp24.E5M2)
+    with pytest.raises(ValueError):
+        sp24.quantize_rows(x.float())
+    with pytest.raises(ValueError):
+        sp24.swiglu_quant(x, x.half())
+    with pytest.raises(ValueError):
+        sp24.gemm_scaled(x, x, x)
+    with pytest.raises(ValueError):
+        sp24.ffn_gated(x, x.half(), x)
+    with pytest.raises(ValueError):
+        sp24.ffn_gated_backward(x.half(), x, x, x, x)
