@@ -330,7 +330,7 @@ sp24_status sp24_gemm_scaled(const sp24_scaled_desc* d, sp24_stream_t stream);
    the backward pass in fp32 through `saved`.  dg and du are rounded to dtype
    (they are tensor-core operands); every output is rounded once.
    x, w_gate and w_up rows must start on 16-byte boundaries (SP24_ERR_ALIGN);
-   so must saved and workspace.  out, d_out and the gradients have no alignment
+   so must the workspace, and saved on a 32-byte one.  out, d_out and the gradients have no alignment
    rule. */
 typedef struct sp24_ffn_desc {
   sp24_dtype dtype;            /* SP24_F16 or SP24_BF16: every tensor below */

@@ -1,0 +1,453 @@
+// sp24_ffn_kernel.cuh — the gated feed-forward block's products on CTA pairs:
+// dense 16-bit operands, tcgen05.mma.cta_group::2 with M = 256, N = 256,
+// fp32 accumulators in TMEM.
+//
+//   kFfnForward  act(x Wg^T) * (x Wu^T): tokens along M, 128 features of Wg and
+//                the same 128 of Wu along N.  CTA 0 of the pair stages Wg's
+//                rows and CTA 1 Wu's, so one MMA fills columns 0-127 of the
+//                accumulator with g and columns 128-255 with u: every epilogue
+//                thread holds both sums of its elements, and no second pass
+//                over x or over h is needed.
+//   kFfnDx       [dg | du] [Wg; Wu]: K runs through f twice, first dg with Wg,
+//                then du with Wu, into one accumulator.
+//   kFfnDw       dg^T x and du^T x: M runs through f twice (one output each),
+//                K through the tokens.
+//
+// Operands are read where they lie: K-major rows (x and W forward, dg forward
+// of Wg) or, where the summed index is the row, MN-major (W in dx, dg and x in
+// dw), in SWIZZLE_128B boxes of 64 x 64 elements; no transposed copy is made.
+// Rows and columns past the end are zero-filled by TMA and not stored.
+//
+// Roles per CTA (11 warps), as in the 2:4 pair kernel (sp24_gemm2sm_kernel.cuh):
+// warps 0 and 10 load A and B, warp 1 of the leader issues the MMAs, warps 2-9
+// drain the accumulator.  It is double-buffered (2 x 256 columns fill TMEM), so
+// a tile's epilogue overlaps the next tile's products.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "sp24_gemm2sm_kernel.cuh"
+#include "sp24_ptx.cuh"
+#include "sp24_rows.cuh"
+
+namespace sp24 {
+
+enum : int { kFfnForward = 0, kFfnDx = 1, kFfnDw = 2 };
+
+struct FfnParams {
+  int m, n;                // rows of a plane's output, output columns (forward: f)
+  int m_tiles, n_tiles;    // of the whole launch (dw: both planes' row tiles)
+  int k_stages;            // 64-deep stages of one tile
+  int plane;               // dx: stages per plane; dw: row tiles per plane
+  int group_m;
+  void *out0, *out1;       // dw: dw_gate, dw_up; else out0
+  long long ld_out0, ld_out1;
+  int vec_out;             // 2: rows start on 32 bytes, 1: on 16, 0: neither
+  float* saved;            // forward: planes g and u, m x ld_saved each, or null
+  long long ld_saved;
+  int silu;
+  int* status;
+  unsigned long long timeout_ns;
+};
+
+// Dense MMA of a CTA pair, both operands from shared memory.
+SP24_DEV void tc_mma_dense_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor, dense kind::f16 with fp32 accumulation (fields as in
+// make_idesc_sparse, plus A's major bit).
+__host__ __device__ constexpr uint32_t make_idesc_dense(uint32_t fmt, uint32_t n, uint32_t m,
+                                                        bool a_mn_major, bool b_mn_major) {
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((a_mn_major ? 1u : 0u) << 15) |
+         ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+template <int DT, int MODE>
+struct FfnCfg {
+  static constexpr bool A_MN = MODE == kFfnDw;
+  static constexpr bool B_MN = MODE != kFfnForward;
+  static constexpr int BK = 64;                       // elements of K per stage
+  static constexpr int OPERAND = 128 * BK * 2;        // 16 KB: this CTA's 128 rows of A or B
+  static constexpr int STAGE_BYTES = 2 * OPERAND;
+  static constexpr int STAGES = 7;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
+  // MN-major boxes hold 64 of the 128 rows: two of them, 8 KB apart.
+  static constexpr int A_BOXES = A_MN ? 2 : 1;
+  static constexpr int B_BOXES = B_MN ? 2 : 1;
+  static constexpr uint32_t A_LBO = A_MN ? OPERAND / 2 : 16;
+  static constexpr uint32_t B_LBO = B_MN ? OPERAND / 2 : 16;
+  // Bytes from one MMA's operand (16 of K) to the next: 16 rows of 128 bytes,
+  // or 32 bytes along a row.
+  static constexpr uint32_t A_STEP = A_MN ? 16 * 128 : 32;
+  static constexpr uint32_t B_STEP = B_MN ? 16 * 128 : 32;
+  static constexpr uint32_t IDESC = make_idesc_dense(DT == 1 ? 1 : 0, 256, 256, A_MN, B_MN);
+  static constexpr int TILE_N = MODE == kFfnForward ? 128 : 256;   // output columns of a tile
+};
+
+template <int DT>
+SP24_DEV uint32_t pack16(float lo, float hi) {
+  if constexpr (DT == 0) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// Warp-collective: 64 consecutive 16-bit columns of the lane's own row, as 32
+// words of two; the warp's rows are row0 .. row0 + 31 and rows >= m are absent.
+// Full runs on 16-byte rows leave as 128-byte pieces through the quad
+// transpose (sp24_gemm2sm_kernel.cuh); the rest goes element by element.
+SP24_DEV void store_run64(void* out, long long ld, int vec, uint32_t (&u)[32], int row0, int m,
+                          int col0, int n) {
+  const int lane = threadIdx.x & 31;
+  if (vec > 0 && col0 + 64 <= n) {
+    quad_transpose_units(u);
+    const int p = lane & 3, g = lane >> 2;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int row = row0 + 4 * g + q;
+      if (row < m) {
+        uint16_t* dst = static_cast<uint16_t*>(out) + row * ld + col0 + 16 * p;
+        if (vec == 2) {
+          st_global_v8_u32(dst, &u[8 * q]);
+        } else {
+          *reinterpret_cast<uint4*>(dst) = make_uint4(u[8 * q], u[8 * q + 1], u[8 * q + 2], u[8 * q + 3]);
+          *reinterpret_cast<uint4*>(dst + 8) =
+              make_uint4(u[8 * q + 4], u[8 * q + 5], u[8 * q + 6], u[8 * q + 7]);
+        }
+      }
+    }
+  } else if (row0 + lane < m) {
+    uint16_t* dst = static_cast<uint16_t*>(out) + (row0 + lane) * ld + col0;
+#pragma unroll
+    for (int j = 0; j < 64; ++j)
+      if (col0 + j < n) dst[j] = static_cast<uint16_t>(u[j / 2] >> (16 * (j & 1)));
+  }
+}
+
+// The same for 32 fp32 columns on rows that start on 32 bytes.
+SP24_DEV void store_run32_f32(float* out, long long ld, uint32_t (&u)[32], int row0, int m, int col0,
+                              int n) {
+  const int lane = threadIdx.x & 31;
+  if (col0 + 32 <= n) {
+    store_rows_128b(out + col0, ld * 4, u, row0, m, false, 0);
+  } else if (row0 + lane < m) {
+    float* dst = out + (row0 + lane) * ld + col0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < n) dst[j] = __uint_as_float(u[j]);
+  }
+}
+
+SP24_DEV float gate_act(float g, int silu_on) { return silu_on ? silu(g) : g; }
+
+SP24_DEV void ffn_tile(const FfnParams& P, int t, int& mt, int& nt) {
+  const int per_group = P.group_m * P.n_tiles;
+  const int g = t / per_group;
+  const int first = g * P.group_m;
+  const int gm = min(P.m_tiles - first, P.group_m);
+  const int r = t - g * per_group;
+  mt = first + r % gm;
+  nt = r / gm;
+}
+
+// tmA0 / tmA1, tmB0 / tmB1: the operands' two planes (forward: A is x, B0 and B1
+// are Wg and Wu; dx: A planes dg and du, B planes Wg and Wu; dw: A planes dg
+// and du, B is x).
+template <int DT, int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    ffn_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
+                    const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
+                    const FfnParams P) {
+#if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
+  using C = FfnCfg<DT, MODE>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t accf_bar[2];
+  __shared__ __align__(8) uint64_t acce_bar[2];
+  __shared__ __align__(8) uint64_t drain_bar;
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ volatile int abort_sh;
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int prank = static_cast<int>(cluster_ctarank());
+  const bool leader = prank == 0;
+  const int pair = static_cast<int>(blockIdx.x >> 1);
+  const int npairs = static_cast<int>(gridDim.x >> 1);
+  const int num_tiles = P.m_tiles * P.n_tiles;
+  const uint64_t tmo = P.timeout_ns;
+
+  if (threadIdx.x == 0) {
+    abort_sh = 0;
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accf_bar[b], 1);
+      mbar_init(&acce_bar[b], 2 * kPairEpiWarps);
+    }
+    mbar_init(&drain_bar, 1);
+    fence_barrier_init();
+    // Every slot is armed for its first use here and re-armed by the MMA warp
+    // as soon as it has seen it full.  Both CTAs' bytes land on the leader's
+    // barrier; TMA counts zero-filled elements too, so all stages are alike.
+    if (leader)
+      for (int s = 0; s < C::STAGES; ++s) mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA0);
+    tma_prefetch_desc(&tmA1);
+    tma_prefetch_desc(&tmB0);
+    tma_prefetch_desc(&tmB1);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&tmem_base_sh, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_sh;
+  griddep_launch_dependents();
+
+  if (warp == 0 || warp == kPairBWarp) {
+    // ------------------------------------------------------------ producers
+    griddep_wait();
+    const bool is_b = warp == kPairBWarp;
+    const bool mn = is_b ? C::B_MN : C::A_MN;
+    const int boxes = is_b ? C::B_BOXES : C::A_BOXES;
+    const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);
+    const uint32_t off = (is_b ? C::OPERAND : 0) + lane * (C::OPERAND / 2);
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    uint32_t used_mask = 0, used_ph = 0;   // slots of the leader's barrier with copies in flight
+    for (int t = pair; t < num_tiles && ok; t += npairs) {
+      int mt, nt;
+      ffn_tile(P, t, mt, nt);
+      const int mplane = MODE == kFfnDw && mt >= P.plane ? 1 : 0;
+      if (MODE == kFfnDw) mt -= mplane * P.plane;
+      // First row (or, MN-major, first column) of this CTA's 128.
+      const int first = is_b ? (MODE == kFfnForward ? nt * 128 : nt * 256 + prank * 128)
+                             : mt * 256 + prank * 128;
+      for (int ks = 0; ks < P.k_stages; ++ks) {
+        int good = 1;
+        if (lane == 0) good = mbar_wait_fast(&empty_bar[s], ph ^ 1u, &abort_sh, tmo) ? 1 : 0;
+        if (__shfl_sync(0xffffffffu, good, 0) == 0) {
+          ok = false;
+          break;
+        }
+        if (leader && lane == 0) {
+          used_mask |= 1u << s;
+          used_ph = (used_ph & ~(1u << s)) | (ph << s);
+        }
+        if (lane < boxes) {
+          const int kplane = MODE == kFfnDx && ks >= P.plane ? 1 : 0;
+          const int k0 = (ks - kplane * P.plane) * C::BK;
+          const bool second = is_b ? (MODE == kFfnForward ? prank == 1 : kplane == 1)
+                                   : (mplane | kplane) == 1;
+          const CUtensorMap* map = is_b ? (second ? &tmB1 : &tmB0) : (second ? &tmA1 : &tmA0);
+          tma_load_2d_pair(smem + s * C::STAGE_BYTES + off, map, full0 + s * sizeof(uint64_t),
+                           mn ? first + lane * 64 : k0, mn ? k0 : first);
+        }
+        if (++s == C::STAGES) s = 0, ph ^= 1u;
+      }
+    }
+    if (!ok && leader && lane == 0) {
+      // Error path: copies in flight land before the CTA leaves.
+      volatile int dummy = 0;
+      for (int i = 0; i < C::STAGES; ++i)
+        if (used_mask & (1u << i)) mbar_wait(&full_bar[i], (used_ph >> i) & 1u, &dummy, tmo);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader)
+    if (leader) {
+      const uint32_t base = smem_u32(smem);
+      const uint64_t adesc0 = make_sdesc(base, C::A_LBO, 1024, kLayoutSW128);
+      const uint64_t bdesc0 = make_sdesc(base + C::OPERAND, C::B_LBO, 1024, kLayoutSW128);
+      int s = 0, buf = 0;
+      uint32_t ph = 0, aph = 0;
+      bool ok = true, any = false;
+      for (int t = pair; t < num_tiles && ok; t += npairs) {
+        if (!mbar_wait_warp<true>(&acce_bar[buf], aph ^ 1u, &abort_sh, tmo)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem_base + static_cast<uint32_t>(buf * 256);
+        for (int ks = 0; ks < P.k_stages; ++ks) {
+          if (!mbar_wait_warp(&full_bar[s], ph, &abort_sh, tmo)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t so = static_cast<uint64_t>(s * (C::STAGE_BYTES >> 4));
+#pragma unroll
+            for (int j = 0; j < C::BK / 16; ++j)
+              tc_mma_dense_pair(d, adesc0 + so + j * (C::A_STEP >> 4),
+                                bdesc0 + so + j * (C::B_STEP >> 4), C::IDESC,
+                                (ks > 0 || j > 0) ? 1u : 0u);
+            tc_commit_pair(&empty_bar[s], 3);
+          }
+          __syncwarp();
+          any = true;
+          if (++s == C::STAGES) s = 0, ph ^= 1u;
+        }
+        if (!ok) break;
+        if (elect_one()) tc_commit_pair(&accf_bar[buf], 3);
+        __syncwarp();
+        buf ^= 1;
+        if (buf == 0) aph ^= 1u;
+      }
+      if (!ok && any) {
+        volatile int dummy = 0;
+        if (elect_one()) tc_commit_pair(&drain_bar, 1);
+        __syncwarp();
+        if (lane == 0) mbar_wait(&drain_bar, 0, &dummy, tmo);
+        __syncwarp();
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;             // TMEM lane quarter
+    const int half = (warp - 2) >> 2;   // which half of the tile's columns
+    uint32_t acce0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
+    int buf = 0;
+    uint32_t aph = 0;
+    for (int t = pair; t < num_tiles; t += npairs) {
+      int mt, nt;
+      ffn_tile(P, t, mt, nt);
+      const int mplane = MODE == kFfnDw && mt >= P.plane ? 1 : 0;
+      if (MODE == kFfnDw) mt -= mplane * P.plane;
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait_sleepy(&accf_bar[buf], aph, &abort_sh, tmo);
+      if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) == 0) break;
+      tc_fence_after();
+      const int row0 = mt * 256 + prank * 128 + q * 32;
+      const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                          static_cast<uint32_t>(buf * 256);
+      // Two passes: 32 features' g and u (forward), or 64 output columns.
+      uint32_t pk[32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t r0[32], r1[32];
+        const uint32_t c0 = tb + (MODE == kFfnForward ? half * 64 + c * 32 : half * 128 + c * 64);
+        tmem_ld_x32(c0, r0);
+        tmem_ld_x32(c0 + (MODE == kFfnForward ? 128 : 32), r1);
+        tmem_ld_wait(r0);
+        tmem_ld_wait(r1);
+        if (c == 1) {   // all of this warp's columns read: the accumulator is free
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(acce0 + buf * sizeof(uint64_t));
+        }
+        if constexpr (MODE == kFfnForward) {
+          const int col0 = nt * 128 + half * 64;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float h[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              h[e] = gate_act(__uint_as_float(r0[j + e]), P.silu) * __uint_as_float(r1[j + e]);
+            pk[(c * 32 + j) / 2] = pack16<DT>(h[0], h[1]);
+          }
+          if (P.saved != nullptr) {
+            store_run32_f32(P.saved, P.ld_saved, r0, row0, P.m, col0 + c * 32, P.n);
+            store_run32_f32(P.saved + P.m * P.ld_saved, P.ld_saved, r1, row0, P.m, col0 + c * 32, P.n);
+          }
+          if (c == 1) store_run64(P.out0, P.ld_out0, P.vec_out, pk, row0, P.m, col0, P.n);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            pk[j / 2] = pack16<DT>(__uint_as_float(r0[j]), __uint_as_float(r0[j + 1]));
+            pk[16 + j / 2] = pack16<DT>(__uint_as_float(r1[j]), __uint_as_float(r1[j + 1]));
+          }
+          store_run64(mplane ? P.out1 : P.out0, mplane ? P.ld_out1 : P.ld_out0, P.vec_out, pk, row0,
+                      P.m, nt * 256 + half * 128 + c * 64, P.n);
+        }
+      }
+      buf ^= 1;
+      if (buf == 0) aph ^= 1u;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+  if (threadIdx.x == 0 && abort_sh != 0 && P.status != nullptr) atomicExch(P.status, 1);
+#endif
+}
+
+// dg = d_out u act'(g) and du = d_out act(g) from the saved fp32 sums, rounded
+// to 16 bits: eight columns a thread, rows of ld (a multiple of 8) elements.
+// The padding past column f is written too (its inputs are whatever the buffer
+// holds) and never read: the products' tensor maps end at f.
+// VEC: d_out's rows start on 16 bytes and f is a multiple of 8.
+template <int DT, int VEC>
+__global__ void __launch_bounds__(256)
+    ffn_dgate_kernel(int t, int f, const float* __restrict__ saved, long long ld,
+                     const void* __restrict__ d_out, long long ldd, int silu_on,
+                     uint16_t* __restrict__ dgu) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const long long per_row = ld / 8, total = per_row * t, plane = ld * t;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+    const long long row = i / per_row;
+    const int col = static_cast<int>(i - row * per_row) * 8;
+    const float* gp = saved + row * ld + col;
+    float g[8], u[8], d[8];
+    *reinterpret_cast<float4*>(g) = *reinterpret_cast<const float4*>(gp);
+    *reinterpret_cast<float4*>(g + 4) = *reinterpret_cast<const float4*>(gp + 4);
+    *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(gp + plane);
+    *reinterpret_cast<float4*>(u + 4) = *reinterpret_cast<const float4*>(gp + plane + 4);
+    if constexpr (VEC) {
+      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(d_out) + row * ldd + col);
+      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] = load16<DT>(&ws[j / 2], j & 1);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] = col + j < f ? load16<DT>(d_out, row * ldd + col + j) : 0.0f;
+    }
+    uint32_t og[4], ou[4];
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      float dg[2], du[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x = g[j + e];
+        const float sg = 1.0f / (1.0f + __expf(-x));
+        du[e] = d[j + e] * (silu_on ? x * sg : x);
+        dg[e] = d[j + e] * u[j + e] * (silu_on ? sg * (1.0f + x * (1.0f - sg)) : 1.0f);
+      }
+      og[j / 2] = pack16<DT>(dg[0], dg[1]);
+      ou[j / 2] = pack16<DT>(du[0], du[1]);
+    }
+    uint16_t* o = dgu + row * ld + col;
+    *reinterpret_cast<uint4*>(o) = make_uint4(og[0], og[1], og[2], og[3]);
+    *reinterpret_cast<uint4*>(o + plane) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+  }
+}
+
+}  // namespace sp24

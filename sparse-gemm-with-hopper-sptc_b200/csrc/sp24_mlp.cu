@@ -1,6 +1,9 @@
 // sp24_mlp.cu — C ABI of the MLP-block operators declared in include/sp24.h:
 // argument checks and launches of the row kernels (sp24_rows.cuh), the 8-bit
 // scaled product and the gated feed-forward block.
+#include <algorithm>
+
+#include "sp24_ffn_kernel.cuh"
 #include "sp24_host.cuh"
 #include "sp24_mlp_simple.cuh"
 #include "sp24_rows.cuh"
@@ -110,17 +113,112 @@ sp24_status check_ffn(const sp24_ffn_desc* d) {
   if (d->w_gate == nullptr || d->w_up == nullptr || (d->t > 0 && d->x == nullptr))
     return SP24_ERR_ARG;
   if (!aligned16(d->x) || !aligned16(d->w_gate) || !aligned16(d->w_up) || ldx % 8 || ldg % 8 ||
-      ldu % 8 || !aligned16(d->saved))
+      ldu % 8 || !aligned32(d->saved))
     return SP24_ERR_ALIGN;
   return SP24_OK;
 }
 
-template <int DT, int GATED>
-sp24_status launch_ffn_simple(const sp24::FfnSimpleParams& p, cudaStream_t s) {
-  const dim3 grid((p.nj + 15) / 16, (p.ni + 15) / 16);
-  sp24::ffn_simple_kernel<DT, GATED><<<grid, 256, 0, s>>>(p);
-  SP24_CUDA_TRY(cudaGetLastError());
-  return SP24_OK;
+// What the three products of a call share.
+struct FfnCall {
+  int sm_count;
+  int* status;
+  cudaStream_t stream;
+};
+
+int out_vec(const void* p, int64_t ld) {
+  return aligned32(p) && ld % 16 == 0 ? 2 : aligned16(p) && ld % 8 == 0 ? 1 : 0;
+}
+
+template <int DT, int MODE>
+sp24_status launch_ffn_pair(const FfnCall& c, const CUtensorMap (&a)[2], const CUtensorMap (&b)[2],
+                            sp24::FfnParams p) {
+  using C = sp24::FfnCfg<DT, MODE>;
+  auto kern = sp24::ffn_pair_kernel<DT, MODE>;
+  static std::atomic<bool> attr_set[kMaxDevices];
+  const sp24_status st = ensure_kernel_attrs(kern, attr_set, C::SMEM_BYTES);
+  if (st != SP24_OK) return st;
+  p.status = c.status;
+  p.timeout_ns = kDefaultTimeoutNs;
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  if (tiles > 0x7fffffff / 2) return SP24_ERR_SHAPE;
+  const unsigned pairs = static_cast<unsigned>(std::min<long long>(tiles, c.sm_count / 2));
+  return launch_gemm_kernel(kern, 2 * pairs, sp24::kPairThreads, C::SMEM_BYTES, c.stream, 0, true,
+                            a[0], a[1], b[0], b[1], p);
+}
+
+// Tensor map of a 16-bit matrix in boxes of 64 columns (128 bytes).
+sp24_status encode_16(CUtensorMap* map, const void* base, int rows, int cols, int64_t ld, int box_rows) {
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, static_cast<uint64_t>(cols),
+                   static_cast<uint64_t>(rows), static_cast<uint64_t>(ld) * 2, 64,
+                   static_cast<uint32_t>(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int DT>
+sp24_status ffn_forward(const FfnCall& c, const sp24_ffn_desc* d, void* out, int64_t ld_out) {
+  CUtensorMap a[2], b[2];
+  sp24_status st = encode_16(&a[0], d->x, d->t, d->h, stride_or(d->ldx, d->h), 128);
+  if (st == SP24_OK) st = encode_16(&b[0], d->w_gate, d->f, d->h, stride_or(d->ld_gate, d->h), 128);
+  if (st == SP24_OK) st = encode_16(&b[1], d->w_up, d->f, d->h, stride_or(d->ld_up, d->h), 128);
+  if (st != SP24_OK) return st;
+  a[1] = a[0];
+  sp24::FfnParams p{};
+  p.m = d->t, p.n = d->f;
+  p.m_tiles = (d->t + 255) / 256, p.n_tiles = (d->f + 127) / 128;
+  p.k_stages = (d->h + 63) / 64;
+  p.group_m = 8;
+  p.out0 = out, p.ld_out0 = ld_out, p.vec_out = out_vec(out, ld_out);
+  p.saved = static_cast<float*>(d->saved), p.ld_saved = ffn_ld(d->f);
+  p.silu = d->act == SP24_ACT_SILU;
+  return launch_ffn_pair<DT, sp24::kFfnForward>(c, a, b, p);
+}
+
+template <int DT>
+sp24_status ffn_backward(const FfnCall& c, const sp24_ffn_desc* d, const sp24_ffn_grads* g) {
+  const int64_t ldw = ffn_ld(d->f), ldd = stride_or(g->ld_d_out, d->f);
+  uint16_t* dg = static_cast<uint16_t*>(g->workspace);
+  uint16_t* du = dg + static_cast<size_t>(d->t) * ldw;
+  const long long chunks = d->t * (ldw / 8);
+  const unsigned grid = static_cast<unsigned>(std::min<long long>((chunks + 255) / 256, c.sm_count * 8));
+  const bool vec = aligned16(g->d_out) && ldd % 8 == 0 && d->f % 8 == 0;
+  auto kern = vec ? sp24::ffn_dgate_kernel<DT, 1> : sp24::ffn_dgate_kernel<DT, 0>;
+  sp24_status st = launch_gemm_kernel(kern, grid, 256, 0, c.stream, 0, true, d->t, d->f,
+                                      static_cast<const float*>(d->saved), static_cast<long long>(ldw),
+                                      static_cast<const void*>(g->d_out), static_cast<long long>(ldd),
+                                      d->act == SP24_ACT_SILU ? 1 : 0, dg);
+  if (st != SP24_OK) return st;
+  CUtensorMap a[2], b[2];
+  if (g->dx != nullptr) {
+    st = encode_16(&a[0], dg, d->t, d->f, ldw, 128);
+    if (st == SP24_OK) st = encode_16(&a[1], du, d->t, d->f, ldw, 128);
+    if (st == SP24_OK) st = encode_16(&b[0], d->w_gate, d->f, d->h, stride_or(d->ld_gate, d->h), 64);
+    if (st == SP24_OK) st = encode_16(&b[1], d->w_up, d->f, d->h, stride_or(d->ld_up, d->h), 64);
+    if (st != SP24_OK) return st;
+    sp24::FfnParams p{};
+    p.m = d->t, p.n = d->h;
+    p.m_tiles = (d->t + 255) / 256, p.n_tiles = (d->h + 255) / 256;
+    p.plane = (d->f + 63) / 64, p.k_stages = 2 * p.plane;
+    p.group_m = 8;
+    p.out0 = g->dx, p.ld_out0 = stride_or(g->ld_dx, d->h), p.vec_out = out_vec(g->dx, p.ld_out0);
+    st = launch_ffn_pair<DT, sp24::kFfnDx>(c, a, b, p);
+    if (st != SP24_OK) return st;
+  }
+  if (g->dw_gate != nullptr) {
+    st = encode_16(&a[0], dg, d->t, d->f, ldw, 64);
+    if (st == SP24_OK) st = encode_16(&a[1], du, d->t, d->f, ldw, 64);
+    if (st == SP24_OK) st = encode_16(&b[0], d->x, d->t, d->h, stride_or(d->ldx, d->h), 64);
+    if (st != SP24_OK) return st;
+    b[1] = b[0];
+    sp24::FfnParams p{};
+    p.m = d->f, p.n = d->h;
+    p.plane = (d->f + 255) / 256, p.m_tiles = 2 * p.plane, p.n_tiles = (d->h + 255) / 256;
+    p.k_stages = (d->t + 63) / 64;
+    p.group_m = 8;
+    p.out0 = g->dw_gate, p.ld_out0 = stride_or(g->ld_dgate, d->h);
+    p.out1 = g->dw_up, p.ld_out1 = stride_or(g->ld_dup, d->h);
+    p.vec_out = std::min(out_vec(p.out0, p.ld_out0), out_vec(p.out1, p.ld_out1));
+    st = launch_ffn_pair<DT, sp24::kFfnDw>(c, a, b, p);
+  }
+  return st;
 }
 
 }  // namespace
@@ -185,15 +283,8 @@ sp24_status sp24_ffn_forward(const sp24_ffn_desc* d, void* out, int64_t ld_out,
   DeviceInfo* di = nullptr;
   st = device_info(&di);
   if (st != SP24_OK) return st;
-  sp24::FfnSimpleParams p{};
-  p.ni = d->t, p.nj = d->f, p.nk = d->h, p.pairs = 1;
-  p.a[0] = d->x, p.b[0] = d->w_gate, p.b[1] = d->w_up;
-  p.a_i = stride_or(d->ldx, d->h), p.a_k = 1, p.b_k = 1, p.b_j = stride_or(d->ld_gate, d->h);
-  p.out = out, p.ldo = ld_out;
-  p.saved = static_cast<float*>(d->saved), p.ld_saved = ffn_ld(d->f);
-  p.silu = d->act == SP24_ACT_SILU;
-  return d->dtype == SP24_F16 ? launch_ffn_simple<0, 1>(p, as_stream(stream))
-                              : launch_ffn_simple<1, 1>(p, as_stream(stream));
+  const FfnCall c{di->sm_count, d->status_dev ? d->status_dev : di->status_word, as_stream(stream)};
+  return d->dtype == SP24_F16 ? ffn_forward<0>(c, d, out, ld_out) : ffn_forward<1>(c, d, out, ld_out);
 }
 
 sp24_status sp24_ffn_backward(const sp24_ffn_desc* d, const sp24_ffn_grads* g,
@@ -223,37 +314,8 @@ sp24_status sp24_ffn_backward(const sp24_ffn_desc* d, const sp24_ffn_grads* g,
     }
     return SP24_OK;
   }
-  const bool f16 = d->dtype == SP24_F16;
-  const int64_t ldw = ffn_ld(d->f);
-  uint16_t* dg = static_cast<uint16_t*>(g->workspace);
-  uint16_t* du = dg + static_cast<size_t>(d->t) * ldw;
-  const dim3 eg((d->f + 255) / 256, d->t);
-  const int silu = d->act == SP24_ACT_SILU;
-  if (f16)
-    sp24::ffn_dgate_kernel<0><<<eg, 256, 0, s>>>(d->t, d->f, static_cast<const float*>(d->saved),
-                                                 ldw, g->d_out, ldd, silu, dg, ldw);
-  else
-    sp24::ffn_dgate_kernel<1><<<eg, 256, 0, s>>>(d->t, d->f, static_cast<const float*>(d->saved),
-                                                 ldw, g->d_out, ldd, silu, dg, ldw);
-  SP24_CUDA_TRY(cudaGetLastError());
-  sp24::FfnSimpleParams p{};
-  if (g->dx != nullptr) {
-    p.ni = d->t, p.nj = d->h, p.nk = d->f, p.pairs = 2;
-    p.a[0] = dg, p.a[1] = du, p.b[0] = d->w_gate, p.b[1] = d->w_up;
-    p.a_i = ldw, p.a_k = 1, p.b_k = stride_or(d->ld_gate, d->h), p.b_j = 1;
-    p.out = g->dx, p.ldo = lddx;
-    st = f16 ? launch_ffn_simple<0, 0>(p, s) : launch_ffn_simple<1, 0>(p, s);
-    if (st != SP24_OK) return st;
-  }
-  for (int w = 0; w < 2 && g->dw_gate != nullptr; ++w) {
-    p.ni = d->f, p.nj = d->h, p.nk = d->t, p.pairs = 1;
-    p.a[0] = w ? du : dg, p.b[0] = d->x;
-    p.a_i = 1, p.a_k = ldw, p.b_k = stride_or(d->ldx, d->h), p.b_j = 1;
-    p.out = w ? g->dw_up : g->dw_gate, p.ldo = w ? ldu : ldg;
-    st = f16 ? launch_ffn_simple<0, 0>(p, s) : launch_ffn_simple<1, 0>(p, s);
-    if (st != SP24_OK) return st;
-  }
-  return SP24_OK;
+  const FfnCall c{di->sm_count, d->status_dev ? d->status_dev : di->status_word, s};
+  return d->dtype == SP24_F16 ? ffn_backward<0>(c, d, g) : ffn_backward<1>(c, d, g);
 }
 
 }  // extern "C"

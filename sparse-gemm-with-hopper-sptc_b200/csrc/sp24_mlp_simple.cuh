@@ -1,5 +1,5 @@
-// sp24_mlp_simple.cuh — plain tiled products of the MLP block on the CUDA
-// cores: one thread per output, operands staged in shared memory.
+// sp24_mlp_simple.cuh — the plain tiled scaled product on the CUDA cores: one
+// thread per output, operands staged in shared memory.
 #pragma once
 
 #include "sp24_rows.cuh"
@@ -64,67 +64,6 @@ __global__ void __launch_bounds__(256) scaled_simple_kernel(const ScaledParams P
   if (P.cdtype == 0) store16<0>(P.c, o, v);
   else if (P.cdtype == 1) store16<1>(P.c, o, v);
   else static_cast<float*>(P.c)[o] = v;
-}
-
-// out(i, j) = sum_k A(i, k) B(k, j) over up to two operand pairs, with any
-// strides; GATED: out = act(sum A B0) * (sum A B1), both sums saved on request.
-struct FfnSimpleParams {
-  int ni, nj, nk, pairs;
-  const void *a[2], *b[2];
-  long long a_i, a_k, b_k, b_j;
-  void* out;
-  long long ldo;
-  float* saved;        // gated: planes of ni x ld_saved
-  long long ld_saved;
-  int silu;
-};
-
-template <int DT, int GATED>
-__global__ void __launch_bounds__(256) ffn_simple_kernel(const FfnSimpleParams P) {
-  __shared__ float as[16][17], b0[16][17], b1[16][17];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const long long i = blockIdx.y * 16LL + ty, j = blockIdx.x * 16LL + tx;
-  float s0 = 0.0f, s1 = 0.0f;
-  for (int p = 0; p < (GATED ? 1 : P.pairs); ++p)
-    for (int k0 = 0; k0 < P.nk; k0 += 16) {
-      const int ka = k0 + tx, kb = k0 + ty;
-      as[ty][tx] = i < P.ni && ka < P.nk ? load16<DT>(P.a[p], i * P.a_i + ka * P.a_k) : 0.0f;
-      const bool in = kb < P.nk && j < P.nj;
-      b0[ty][tx] = in ? load16<DT>(P.b[p], kb * P.b_k + j * P.b_j) : 0.0f;
-      if (GATED) b1[ty][tx] = in ? load16<DT>(P.b[1], kb * P.b_k + j * P.b_j) : 0.0f;
-      __syncthreads();
-      for (int k = 0; k < 16; ++k) {
-        s0 += as[ty][k] * b0[k][tx];
-        if (GATED) s1 += as[ty][k] * b1[k][tx];
-      }
-      __syncthreads();
-    }
-  if (i >= P.ni || j >= P.nj) return;
-  if (GATED) {
-    if (P.saved) {
-      P.saved[i * P.ld_saved + j] = s0;
-      P.saved[(P.ni + i) * P.ld_saved + j] = s1;
-    }
-    s0 = (P.silu ? s0 / (1.0f + __expf(-s0)) : s0) * s1;
-  }
-  store16<DT>(P.out, i * P.ldo + j, s0);
-}
-
-// dg and du from d_out and the saved sums.
-template <int DT>
-__global__ void __launch_bounds__(256)
-    ffn_dgate_kernel(int t, int f, const float* saved, long long ld_saved, const void* d_out,
-                     long long ldd, int silu, void* dgu, long long ldw) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  const long long i = blockIdx.y;
-  if (j >= f) return;
-  const float g = saved[i * ld_saved + j], u = saved[(t + i) * ld_saved + j];
-  const float d = load16<DT>(d_out, i * ldd + j);
-  const float sg = 1.0f / (1.0f + __expf(-g));
-  const float a = silu ? g * sg : g;
-  const float da = silu ? sg * (1.0f + g * (1.0f - sg)) : 1.0f;
-  store16<DT>(dgu, i * ldw + j, d * u * da);
-  store16<DT>(dgu, (t + i) * ldw + j, d * a);
 }
 
 }  // namespace sp24
