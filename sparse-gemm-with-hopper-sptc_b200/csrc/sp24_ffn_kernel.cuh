@@ -92,17 +92,6 @@ struct FfnCfg {
   static constexpr int TILE_N = MODE == kFfnForward ? 128 : 256;   // output columns of a tile
 };
 
-template <int DT>
-SP24_DEV uint32_t pack16(float lo, float hi) {
-  if constexpr (DT == 0) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-
 // Warp-collective: 64 consecutive 16-bit columns of the lane's own row, as 32
 // words of two; the warp's rows are row0 .. row0 + 31 and rows >= m are absent.
 // Full runs on 16-byte rows leave as 128-byte pieces through the quad

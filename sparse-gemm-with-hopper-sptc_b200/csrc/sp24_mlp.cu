@@ -57,11 +57,38 @@ sp24_status check_rows(const sp24_rowquant_desc* d, int mode, sp24::RowsParams* 
   return SP24_OK;
 }
 
+template <int DT, int MODE, int I8, int V, int VPT>
+sp24_status launch_rows_vpt(const sp24::RowsParams& p, int vecs, cudaStream_t s) {
+  if (vecs <= 32 * VPT) {
+    const unsigned per_block = 8;
+    return launch_gemm_kernel(sp24::rows_quant_kernel<DT, MODE, I8, V, VPT, true>,
+                              (p.rows + per_block - 1) / per_block, 32 * per_block, 0, s, 0, true, p);
+  }
+  const unsigned threads = static_cast<unsigned>(round_up((vecs + VPT - 1) / VPT, 32));
+  return launch_gemm_kernel(sp24::rows_quant_kernel<DT, MODE, I8, V, VPT, false>,
+                            static_cast<unsigned>(p.rows), threads, 0, s, 0, true, p);
+}
+
+// Vectors a thread holds.  Many rows: four, so that a row's reductions span few
+// warps and several rows share an SM.  Few rows (up to two blocks an SM): one,
+// so that a row's loads spread over as many threads as there are.
+template <int DT, int MODE, int I8, int V>
+sp24_status launch_rows_v(const sp24::RowsParams& p, const DeviceInfo& di, cudaStream_t s) {
+  const int vecs = (p.cols + V - 1) / V;
+  const bool few = p.rows <= 2 * di.sm_count;
+  if (few && vecs <= 1024) return launch_rows_vpt<DT, MODE, I8, V, 1>(p, vecs, s);
+  if (vecs <= 4 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 4>(p, vecs, s);
+  return launch_gemm_kernel(sp24::rows_quant_long_kernel<DT, MODE, I8>,
+                            static_cast<unsigned>(p.rows), 1024, 0, s, 0, true, p);
+}
+
 template <int DT, int MODE, int I8>
-sp24_status launch_rows(const sp24::RowsParams& p, cudaStream_t s) {
-  sp24::rows_quant_kernel<DT, MODE, I8><<<static_cast<unsigned>(p.rows), 256, 0, s>>>(p);
-  SP24_CUDA_TRY(cudaGetLastError());
-  return SP24_OK;
+sp24_status launch_rows(const sp24::RowsParams& p, const DeviceInfo& di, cudaStream_t s) {
+  auto vec = [](const void* q, long long ld) { return q == nullptr || (aligned16(q) && ld % 8 == 0); };
+  const bool v8 = p.cols % 8 == 0 && vec(p.x, p.ldx) && vec(p.up, p.ld_up) &&
+                  vec(p.residual, p.ld_residual) && vec(p.residual_out, p.ld_residual_out) &&
+                  vec(p.weight, 0) && reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && p.ldq % 8 == 0;
+  return v8 ? launch_rows_v<DT, MODE, I8, 8>(p, di, s) : launch_rows_v<DT, MODE, I8, 1>(p, di, s);
 }
 
 template <int MODE>
@@ -75,8 +102,8 @@ sp24_status rows_quant(const sp24_rowquant_desc* d, sp24_stream_t stream) {
   cudaStream_t s = as_stream(stream);
   const bool i8 = d->qdtype == SP24_I8;
   if (d->dtype == SP24_F16)
-    return i8 ? launch_rows<0, MODE, 1>(p, s) : launch_rows<0, MODE, 0>(p, s);
-  return i8 ? launch_rows<1, MODE, 1>(p, s) : launch_rows<1, MODE, 0>(p, s);
+    return i8 ? launch_rows<0, MODE, 1>(p, *di, s) : launch_rows<0, MODE, 0>(p, *di, s);
+  return i8 ? launch_rows<1, MODE, 1>(p, *di, s) : launch_rows<1, MODE, 0>(p, *di, s);
 }
 
 // ------------------------------------------------------------------ scaled product

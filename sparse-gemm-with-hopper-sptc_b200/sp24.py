@@ -381,12 +381,14 @@ def gemm_fused(a_c, meta, b, m, n, k, *, bias=None, act=ACT_NONE, a_c_up=None, m
 
 def _rows2d(t, what, cols=None, rows=None):
     """A CUDA matrix whose rows are contiguous (any row stride)."""
-    if not t.is_cuda or t.dim() != 2:
-        raise ValueError(f"{what}: a 2-D CUDA tensor is wanted")
-    if (cols is not None and t.shape[1] != cols) or (rows is not None and t.shape[0] != rows):
+    if t.dim() != 2:
+        raise ValueError(f"{what}: a 2-D tensor is wanted")
+    r, c = t.shape
+    if (cols is not None and c != cols) or (rows is not None and r != rows):
         raise ValueError(f"{what}: shape {tuple(t.shape)}, expected "
                          f"({'any' if rows is None else rows}, {'any' if cols is None else cols})")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1] or (t.shape[1] > 1 and t.stride(1) != 1):
+    ld, step = t.stride()
+    if r > 1 and ld < c or c > 1 and step != 1:
         t = t.contiguous()
     return t
 
@@ -415,34 +417,43 @@ def _tma_ld(t):
     return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + unit - 1) // unit * unit
 
 
-def _same_device(*ts):
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) != 1:
-        raise ValueError(f"tensors on several devices: {sorted(map(str, devs))}")
-    return devs.pop()
+def _same_device(first, *rest):
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError(f"CUDA tensors are wanted, not {dev}")
+    for t in rest:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on several devices: {dev}, {t.device}")
+    return dev
 
 
 class _On:
     """Work of one call: its device current and its stream torch's current one,
-    so that copies and outputs made on the way are ordered with the kernels."""
+    so that copies and outputs made on the way are ordered with the kernels.
+    Where both already are, nothing is switched (a switch costs several
+    microseconds of host time)."""
+
+    __slots__ = ("ctx", "handle")
 
     def __init__(self, device, stream):
         import torch
-        self.dev = torch.cuda.device(device)
-        self.ctx = torch.cuda.stream(stream) if stream is not None else None
-        self.device = device
+        self.ctx = []
+        if torch.cuda.current_device() != device.index:
+            self.ctx.append(torch.cuda.device(device))
+        if stream is not None:
+            self.ctx.append(torch.cuda.stream(stream))
+            self.handle = stream.cuda_stream
+        else:
+            self.handle = torch._C._cuda_getCurrentRawStream(device.index)
 
     def __enter__(self):
-        import torch
-        self.dev.__enter__()
-        if self.ctx is not None:
-            self.ctx.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
+        for c in self.ctx:
+            c.__enter__()
+        return self.handle
 
     def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-        self.dev.__exit__(*exc)
+        for c in reversed(self.ctx):
+            c.__exit__(*exc)
 
 
 def _quant_dtype(qdtype):
