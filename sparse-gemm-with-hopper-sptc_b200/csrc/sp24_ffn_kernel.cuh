@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float x = g[j + e];
-        const float sg = 1.0f / (1.0f + __expf(-x));
+        const float sg = __fdividef(1.0f, 1.0f + __expf(-x));
         du[e] = d[j + e] * (silu_on ? x * sg : x);
         dg[e] = d[j + e] * u[j + e] * (silu_on ? sg * (1.0f + x * (1.0f - sg)) : 1.0f);
       }

@@ -57,27 +57,59 @@ sp24_status check_rows(const sp24_rowquant_desc* d, int mode, sp24::RowsParams* 
   return SP24_OK;
 }
 
-template <int DT, int MODE, int I8, int V, int VPT>
-sp24_status launch_rows_vpt(const sp24::RowsParams& p, int vecs, cudaStream_t s) {
-  if (vecs <= 32 * VPT) {
-    const unsigned per_block = 8;
-    return launch_gemm_kernel(sp24::rows_quant_kernel<DT, MODE, I8, V, VPT, true>,
-                              (p.rows + per_block - 1) / per_block, 32 * per_block, 0, s, 0, true, p);
+// A resident grid: as many blocks as fit the registers, threads and shared
+// memory of the SMs.
+template <int DT, int MODE, int I8, int V, int VPT, bool ONE_WARP>
+sp24_status launch_rows_kernel(const sp24::RowsParams& p, const DeviceInfo& di, unsigned threads, cudaStream_t s) {
+  constexpr int kSmem = 200 * 1024;   // of an SM, for the slots
+  auto kern = sp24::rows_quant_kernel<DT, MODE, I8, V, VPT, ONE_WARP>;
+  static std::atomic<bool> attr_set[kMaxDevices];
+  static std::atomic<int> regs{0};
+  sp24_status st = ensure_kernel_attrs(kern, attr_set, V == 8 ? 2 * VPT * (ONE_WARP ? 256 : 1024) * 16 : 0);
+  if (st != SP24_OK) return st;
+  if (regs.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes a{};
+    SP24_CUDA_TRY(cudaFuncGetAttributes(&a, kern));
+    regs.store((a.numRegs + 7) / 8 * 8, std::memory_order_relaxed);
   }
-  const unsigned threads = static_cast<unsigned>(round_up((vecs + VPT - 1) / VPT, 32));
-  return launch_gemm_kernel(sp24::rows_quant_kernel<DT, MODE, I8, V, VPT, false>,
-                            static_cast<unsigned>(p.rows), threads, 0, s, 0, true, p);
+  const int inputs = p.up != nullptr || p.residual != nullptr ? 2 : 1;
+  const int smem = V == 8 ? inputs * VPT * static_cast<int>(threads) * 16 : 0;
+  const int t = static_cast<int>(threads);
+  int blocks = std::min({2048 / t, 65536 / (regs.load(std::memory_order_relaxed) * t), 32});
+  if (smem > 0) blocks = std::min(blocks, kSmem / smem);
+  blocks = std::max(blocks, 1);
+  const long long per_block = ONE_WARP ? t / 32 : 1;
+  const long long want = (p.rows + per_block - 1) / per_block;
+  const unsigned grid = static_cast<unsigned>(std::min<long long>(want, static_cast<long long>(blocks) * di.sm_count));
+  return launch_gemm_kernel(kern, grid, threads, smem, s, 0, true, p);
 }
 
-// Vectors a thread holds.  Many rows: four, so that a row's reductions span few
-// warps and several rows share an SM.  Few rows (up to two blocks an SM): one,
-// so that a row's loads spread over as many threads as there are.
+template <int DT, int MODE, int I8, int V, int VPT>
+sp24_status launch_rows_vpt(const sp24::RowsParams& p, const DeviceInfo& di, int vecs, cudaStream_t s) {
+  if (vecs <= 32 * VPT) return launch_rows_kernel<DT, MODE, I8, V, VPT, true>(p, di, 256, s);
+  const unsigned threads = static_cast<unsigned>(round_up((vecs + VPT - 1) / VPT, 32));
+  return launch_rows_kernel<DT, MODE, I8, V, VPT, false>(p, di, threads, s);
+}
+
+// Vectors a thread holds.  A row of up to 32 vectors: one, a warp per row (8192
+// x 256 norm: 6.2 us; 7.5 with two, 10.3 with four).  The norm, with its two
+// barriers a row, wants rows spread over more warps than the others (8192 x
+// 4096: 40.7 us with two, 45.2 with four; plain rows 20.6 and 18.6), and so
+// does a call with few rows, whose loads then go out at once (333 x 5000 norm:
+// 6.4 us with two, 7.9 with four).  Single elements (V = 1) want eight: fewer
+// threads, more loads each (4096 x 1001 swiglu: 12.3 us; 12.9 with four).
 template <int DT, int MODE, int I8, int V>
 sp24_status launch_rows_v(const sp24::RowsParams& p, const DeviceInfo& di, cudaStream_t s) {
   const int vecs = (p.cols + V - 1) / V;
-  const bool few = p.rows <= 2 * di.sm_count;
-  if (few && vecs <= 1024) return launch_rows_vpt<DT, MODE, I8, V, 1>(p, vecs, s);
-  if (vecs <= 4 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 4>(p, vecs, s);
+  if constexpr (V == 8) {
+    if (vecs <= 32) return launch_rows_vpt<DT, MODE, I8, V, 1>(p, di, vecs, s);
+    const bool few = p.rows <= 2 * di.sm_count;
+    if ((MODE == sp24::kRowsNorm || few) && vecs <= 2 * 1024)
+      return launch_rows_vpt<DT, MODE, I8, V, 2>(p, di, vecs, s);
+    if (vecs <= 4 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 4>(p, di, vecs, s);
+  } else {
+    if (vecs <= 8 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 8>(p, di, vecs, s);
+  }
   return launch_gemm_kernel(sp24::rows_quant_long_kernel<DT, MODE, I8>,
                             static_cast<unsigned>(p.rows), 1024, 0, s, 0, true, p);
 }
