@@ -5,8 +5,8 @@
 
 #include "sp24_ffn_kernel.cuh"
 #include "sp24_host.cuh"
-#include "sp24_mlp_simple.cuh"
 #include "sp24_rows.cuh"
+#include "sp24_stream_kernel.cuh"
 
 using namespace sp24host;
 
@@ -212,8 +212,86 @@ sp24_status encode_16(CUtensorMap* map, const void* base, int rows, int cols, in
                    static_cast<uint32_t>(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// ------------------------------------------------------------------ few tokens
+constexpr int kStreamMaxTokens = 128;
+
+template <int OP, int BN>
+sp24_status launch_stream_bn(const FfnCall& c, const CUtensorMap& a, const CUtensorMap& a2,
+                             const CUtensorMap& b, sp24::StreamParams p) {
+  using C = sp24::StreamCfg<OP, BN>;
+  auto kern = sp24::stream_kernel<OP, BN>;
+  static std::atomic<bool> attr_set[kMaxDevices];
+  const sp24_status st = ensure_kernel_attrs(kern, attr_set, C::SMEM_BYTES);
+  if (st != SP24_OK) return st;
+  p.stages = (p.k + C::BKD - 1) / C::BKD;
+  const int n_tiles = (p.n + BN - 1) / BN;
+  const long long tiles = static_cast<long long>(p.m_blocks) * n_tiles;
+  if (tiles * sp24::kStreamMaxSplits > 0x7fffffff) return SP24_ERR_SHAPE;
+  p.splits = static_cast<int>(std::max(1LL, std::min<long long>({c.sm_count / tiles, sp24::kStreamMaxSplits,
+                                                                 p.stages})));
+  p.status = c.status;
+  p.timeout_ns = kDefaultTimeoutNs;
+  return launch_gemm_kernel(kern, static_cast<unsigned>(tiles * p.splits), sp24::kStreamThreads,
+                            C::SMEM_BYTES, c.stream, static_cast<unsigned>(p.splits), true, a, a2, b, p);
+}
+
+// rows of a TMA box of B for n tokens
+inline int stream_bn(int n) { return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+
+template <int OP>
+sp24_status launch_stream(const FfnCall& c, const CUtensorMap& a, const CUtensorMap& a2,
+                          const CUtensorMap& b, const sp24::StreamParams& p) {
+  switch (stream_bn(p.n)) {
+    case 16: return launch_stream_bn<OP, 16>(c, a, a2, b, p);
+    case 32: return launch_stream_bn<OP, 32>(c, a, a2, b, p);
+    case 64: return launch_stream_bn<OP, 64>(c, a, a2, b, p);
+    default: return launch_stream_bn<OP, 128>(c, a, a2, b, p);
+  }
+}
+
+template <int OP>
+sp24_status scaled(const FfnCall& c, const sp24_scaled_desc* d) {
+  CUtensorMap a, b;
+  auto encode_8 = [](CUtensorMap* map, const void* base, int rows, int cols, int64_t ld, int box_rows) {
+    return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, static_cast<uint64_t>(cols),
+                     static_cast<uint64_t>(rows), static_cast<uint64_t>(ld), 128,
+                     static_cast<uint32_t>(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  sp24_status st = encode_8(&a, d->a_c, d->m, d->k / 2, stride_or(d->lda_c, d->k / 2), 128);
+  if (st == SP24_OK) st = encode_8(&b, d->x, d->n, d->k, stride_or(d->ldx, d->k), stream_bn(d->n));
+  if (st != SP24_OK) return st;
+  sp24::StreamParams p{};
+  p.m = d->m, p.n = d->n, p.k = d->k;
+  p.m_blocks = (d->m + 127) / 128;
+  p.meta = d->meta;
+  p.meta_mblocks = meta_mblocks(d->m), p.katoms = meta_katoms(d->k);
+  p.scale_m = d->scale_m, p.scale_n = d->scale_n, p.bias = d->bias;
+  p.out = d->c, p.ldo = stride_or(d->ldc, d->m);
+  p.out_type = d->cdtype == SP24_F32 ? 2 : static_cast<int>(d->cdtype);
+  p.static_weights = (sp24_get_launch_hints() & SP24_HINT_STATIC_WEIGHTS) != 0;
+  return launch_stream<OP>(c, a, a, b, p);
+}
+
+template <int DT>
+sp24_status ffn_forward_few(const FfnCall& c, const sp24_ffn_desc* d, void* out, int64_t ld_out) {
+  CUtensorMap a, a2, b;
+  sp24_status st = encode_16(&a, d->w_gate, d->f, d->h, stride_or(d->ld_gate, d->h), 128);
+  if (st == SP24_OK) st = encode_16(&a2, d->w_up, d->f, d->h, stride_or(d->ld_up, d->h), 128);
+  if (st == SP24_OK) st = encode_16(&b, d->x, d->t, d->h, stride_or(d->ldx, d->h), stream_bn(d->t));
+  if (st != SP24_OK) return st;
+  sp24::StreamParams p{};
+  p.m = d->f, p.n = d->t, p.k = d->h;
+  p.m_blocks = (d->f + 127) / 128;
+  p.out = out, p.ldo = ld_out, p.out_type = DT;
+  p.saved = static_cast<float*>(d->saved), p.ld_saved = ffn_ld(d->f);
+  p.silu = d->act == SP24_ACT_SILU;
+  p.static_weights = (sp24_get_launch_hints() & SP24_HINT_STATIC_WEIGHTS) != 0;
+  return launch_stream<DT == 0 ? sp24::kStreamF16 : sp24::kStreamBF16>(c, a, a2, b, p);
+}
+
 template <int DT>
 sp24_status ffn_forward(const FfnCall& c, const sp24_ffn_desc* d, void* out, int64_t ld_out) {
+  if (d->t <= kStreamMaxTokens) return ffn_forward_few<DT>(c, d, out, ld_out);
   CUtensorMap a[2], b[2];
   sp24_status st = encode_16(&a[0], d->x, d->t, d->h, stride_or(d->ldx, d->h), 128);
   if (st == SP24_OK) st = encode_16(&b[0], d->w_gate, d->f, d->h, stride_or(d->ld_gate, d->h), 128);
@@ -302,23 +380,8 @@ sp24_status sp24_gemm_scaled(const sp24_scaled_desc* d, sp24_stream_t stream) {
   DeviceInfo* di = nullptr;
   st = device_info(&di);
   if (st != SP24_OK) return st;
-  sp24::ScaledParams p{};
-  p.m = d->m, p.n = d->n, p.k = d->k;
-  p.a_c = static_cast<const uint8_t*>(d->a_c);
-  p.lda_c = stride_or(d->lda_c, d->k / 2);
-  p.meta = d->meta;
-  p.meta_mblocks = meta_mblocks(d->m);
-  p.x = static_cast<const uint8_t*>(d->x);
-  p.ldx = stride_or(d->ldx, d->k);
-  p.scale_m = d->scale_m, p.scale_n = d->scale_n, p.bias = d->bias;
-  p.c = d->c;
-  p.ldc = stride_or(d->ldc, d->m);
-  p.cdtype = d->cdtype == SP24_F32 ? 2 : static_cast<int>(d->cdtype);
-  const dim3 grid((d->m + 15) / 16, (d->n + 15) / 16);
-  if (d->dtype == SP24_I8) sp24::scaled_simple_kernel<1><<<grid, 256, 0, as_stream(stream)>>>(p);
-  else sp24::scaled_simple_kernel<0><<<grid, 256, 0, as_stream(stream)>>>(p);
-  SP24_CUDA_TRY(cudaGetLastError());
-  return SP24_OK;
+  const FfnCall c{di->sm_count, d->status_dev ? d->status_dev : di->status_word, as_stream(stream)};
+  return d->dtype == SP24_I8 ? scaled<sp24::kStreamI8>(c, d) : scaled<sp24::kStreamE4M3>(c, d);
 }
 
 size_t sp24_ffn_saved_bytes(int t, int f) {
