@@ -378,9 +378,12 @@ def gemm_fused(a_c, meta, b, m, n, k, *, bias=None, act=ACT_NONE, a_c_up=None, m
 
 # ------------------------------------------------------------------ the MLP block
 # Activations are token-major: one row per token, its features contiguous.
+# These calls serve single tokens, where the host's time is what counts: shapes
+# and strides are read once, and descriptors are built in one go.
 
 def _rows2d(t, what, cols=None, rows=None):
-    """A CUDA matrix whose rows are contiguous (any row stride)."""
+    """(t, row stride) of a matrix whose rows are contiguous, any row stride;
+    others are copied.  A single row's stride says nothing: 0."""
     if t.dim() != 2:
         raise ValueError(f"{what}: a 2-D tensor is wanted")
     r, c = t.shape
@@ -390,31 +393,21 @@ def _rows2d(t, what, cols=None, rows=None):
     ld, step = t.stride()
     if r > 1 and ld < c or c > 1 and step != 1:
         t = t.contiguous()
-    return t
-
-
-def _ld(t):
-    """Row stride in elements; a single row's stride says nothing."""
-    return t.stride(0) if t.shape[0] > 1 else 0
+        ld = c
+    return t, (ld if r > 1 else 0)
 
 
 def _tma_rows(t, what, cols=None, rows=None):
     """_rows2d whose rows also start on 16-byte boundaries (TMA operands):
     others are copied into padded rows first."""
-    t = _rows2d(t, what, cols, rows)
+    t, ld = _rows2d(t, what, cols, rows)
     unit = 16 // t.element_size()
-    if t.data_ptr() % 16 == 0 and (t.shape[0] == 1 and t.shape[1] % unit == 0
-                                   or t.shape[0] > 1 and t.stride(0) % unit == 0):
-        return t
+    if t.data_ptr() % 16 == 0 and (ld or t.shape[1]) % unit == 0:
+        return t, ld
     ld = (t.shape[1] + unit - 1) // unit * unit
     padded = t.new_empty((t.shape[0], ld))[:, :t.shape[1]]
     padded.copy_(t)
-    return padded
-
-
-def _tma_ld(t):
-    unit = 16 // t.element_size()
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + unit - 1) // unit * unit
+    return padded, ld
 
 
 def _same_device(first, *rest):
@@ -424,99 +417,125 @@ def _same_device(first, *rest):
     for t in rest:
         if t is not None and t.device != dev:
             raise ValueError(f"tensors on several devices: {dev}, {t.device}")
-    return dev
+    return dev.index
 
 
-class _On:
-    """Work of one call: its device current and its stream torch's current one,
-    so that copies and outputs made on the way are ordered with the kernels.
-    Where both already are, nothing is switched (a switch costs several
-    microseconds of host time)."""
-
-    __slots__ = ("ctx", "handle")
-
-    def __init__(self, device, stream):
-        import torch
-        self.ctx = []
-        if torch.cuda.current_device() != device.index:
-            self.ctx.append(torch.cuda.device(device))
-        if stream is not None:
-            self.ctx.append(torch.cuda.stream(stream))
-            self.handle = stream.cuda_stream
-        else:
-            self.handle = torch._C._cuda_getCurrentRawStream(device.index)
-
-    def __enter__(self):
-        for c in self.ctx:
-            c.__enter__()
-        return self.handle
-
-    def __exit__(self, *exc):
-        for c in reversed(self.ctx):
-            c.__exit__(*exc)
-
-
-def _quant_dtype(qdtype):
+def _on(index, stream, call, *args):
+    """call(raw stream, *args) with the tensors' device current and `stream`
+    (None: the current one) torch's current stream, so that copies and outputs
+    made on the way are ordered with the kernels."""
     import torch
-    if qdtype == I8:
-        return torch.int8
-    if qdtype == E4M3:
-        return torch.float8_e4m3fn
-    raise ValueError(f"qdtype {qdtype}: I8 or E4M3")
+    if stream is None and torch._C._cuda_getDevice() == index:
+        return call(torch._C._cuda_getCurrentRawStream(index), *args)
+    with torch.cuda.device(index), torch.cuda.stream(stream):
+        return call(torch._C._cuda_getCurrentRawStream(index), *args)
 
 
-def _rows_quant(entry, x, qdtype, stream, up=None, weight=None, residual=None, eps=0.0):
+_codes = {}
+
+
+def _code_tables():
+    """Torch dtype -> library code, by use."""
     import torch
-    lib = load()
-    code_dtype = _quant_dtype(qdtype)
+    _codes["16"] = {torch.float16: F16, torch.bfloat16: BF16}
+    _codes["8"] = {torch.int8: I8, torch.float8_e4m3fn: E4M3}
+    _codes["out"] = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
+    _codes["of_8"] = {I8: torch.int8, E4M3: torch.float8_e4m3fn}
+    return _codes
+
+
+def _rows_quant(s, entry, x, qdtype, up, weight, residual, eps):
+    import torch
+    tables = _codes or _code_tables()
+    dt, q_torch = tables["16"].get(x.dtype), tables["of_8"].get(qdtype)
+    if dt is None:
+        raise ValueError(f"{entry}: float16 or bfloat16 rows, not {x.dtype}")
+    if q_torch is None:
+        raise ValueError(f"{entry}: qdtype {qdtype}, not I8 or E4M3")
     for t in (up, weight, residual):
         if t is not None and t.dtype != x.dtype:
             raise ValueError(f"{entry}: {t.dtype} beside {x.dtype}")
-    if x.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"{entry}: float16 or bfloat16 rows, not {x.dtype}")
-    with _On(_same_device(x, up, weight, residual), stream) as s:
-        x = _rows2d(x, "x")
-        rows, cols = x.shape
-        d = RowQuantDesc()
-        d.dtype, d.qdtype, d.rows, d.cols = dtype_code(x.dtype), qdtype, rows, cols
-        d.x, d.ldx = _ptr(x), _ld(x)
-        if up is not None:
-            up = _rows2d(up, "up", cols, rows)
-            d.up, d.ld_up = _ptr(up), _ld(up)
-        total = None
-        if weight is not None:
-            if weight.shape != (cols,):
-                raise ValueError(f"weight: shape {tuple(weight.shape)}, expected ({cols},)")
-            weight = weight.contiguous()
-            d.weight, d.eps = _ptr(weight), eps
-        if residual is not None:
-            residual = _rows2d(residual, "residual", cols, rows)
-            total = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-            d.residual, d.ld_residual, d.residual_out = _ptr(residual), _ld(residual), _ptr(total)
-        q = torch.empty((rows, cols), dtype=code_dtype, device=x.device)
-        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-        d.q, d.scale = _ptr(q), _ptr(scale)
-        _check(getattr(lib, entry)(ctypes.byref(d), s), entry)
-    return (q, scale) if residual is None else (q, scale, total)
+    x, ldx = _rows2d(x, "x")
+    rows, cols = x.shape
+    total = None
+    ld_up = ld_res = p_up = p_res = p_total = p_weight = 0
+    if up is not None:
+        up, ld_up = _rows2d(up, "up", cols, rows)
+        p_up = up.data_ptr()
+    if weight is not None:
+        if weight.shape != (cols,):
+            raise ValueError(f"weight: shape {tuple(weight.shape)}, expected ({cols},)")
+        weight = weight.contiguous()
+        p_weight = weight.data_ptr()
+    plain = x.is_contiguous()
+    if residual is not None:
+        residual, ld_res = _rows2d(residual, "residual", cols, rows)
+        total = torch.empty_like(x) if plain else x.new_empty((rows, cols))
+        p_res, p_total = residual.data_ptr(), total.data_ptr()
+    q = torch.empty_like(x, dtype=q_torch) if plain else x.new_empty((rows, cols), dtype=q_torch)
+    scale = x.new_empty((rows,), dtype=torch.float32)
+    d = RowQuantDesc(dt, qdtype, rows, cols, x.data_ptr(), ldx, p_up, ld_up, p_res, ld_res,
+                     p_total, 0, p_weight, eps, q.data_ptr(), 0, scale.data_ptr())
+    _check(getattr(_lib or load(), entry)(ctypes.byref(d), s), entry)
+    return (q, scale) if total is None else (q, scale, total)
 
 
 def rmsnorm_quant(x, weight, residual=None, *, eps=1e-6, qdtype=I8, stream=None):
     """sp24_rmsnorm_quant: 8-bit rows of rmsnorm(x [+ residual]) * weight.
     Returns (q, scale), or (q, scale, x + residual) when a residual is given;
     a row's values are q * scale."""
-    return _rows_quant("sp24_rmsnorm_quant", x, qdtype, stream, weight=weight, residual=residual,
-                       eps=eps)
+    return _on(_same_device(x, weight, residual), stream, _rows_quant, "sp24_rmsnorm_quant", x,
+               qdtype, None, weight, residual, eps)
 
 
 def swiglu_quant(gate, up, *, qdtype=I8, stream=None):
     """sp24_swiglu_quant: 8-bit rows of silu(gate) * up -> (q, scale)."""
-    return _rows_quant("sp24_swiglu_quant", gate, qdtype, stream, up=up)
+    return _on(_same_device(gate, up), stream, _rows_quant, "sp24_swiglu_quant", gate, qdtype, up,
+               None, None, 0.0)
 
 
 def quantize_rows(x, *, qdtype=I8, stream=None):
     """sp24_quantize_rows: 8-bit rows of x -> (q, scale).  Applied to a 16-bit
     A_c it gives the 8-bit weights of gemm_scaled and their channel scales."""
-    return _rows_quant("sp24_quantize_rows", x, qdtype, stream)
+    return _on(_same_device(x), stream, _rows_quant, "sp24_quantize_rows", x, qdtype, None, None,
+               None, 0.0)
+
+
+def _vector_f32(t, size, what):
+    """(tensor to keep, pointer) of an optional vector of `size` floats."""
+    import torch
+    if t is None:
+        return None, 0
+    if t.dtype != torch.float32 or t.numel() != size:
+        raise ValueError(f"{what}: {size} float32 values are wanted")
+    t = t.contiguous()
+    return t, t.data_ptr()
+
+
+def _gemm_scaled(s, a_c, meta_tc, x, scale_w, scale_x, bias, out_dtype):
+    import torch
+    lib = _lib or load()
+    tables = _codes or _code_tables()
+    code, out = tables["8"].get(x.dtype), tables["out"].get(out_dtype or torch.bfloat16)
+    if code is None or a_c.dtype != x.dtype:
+        raise ValueError(f"gemm_scaled: {x.dtype} tokens and {a_c.dtype} weights; both int8 or "
+                         "both float8_e4m3fn are wanted")
+    if out is None:
+        raise ValueError(f"gemm_scaled: out_dtype {out_dtype}")
+    a_c, lda = _tma_rows(a_c, "a_c")
+    m, k = a_c.shape[0], 2 * a_c.shape[1]
+    x, ldx = _tma_rows(x, "x", k)
+    n = x.shape[0]
+    if meta_tc.nbytes != lib.sp24_meta_tc_bytes(m, k):
+        raise ValueError(f"meta_tc: {meta_tc.nbytes} bytes, {meta_tc_bytes(m, k)} expected")
+    scale_w, p_w = _vector_f32(scale_w, m, "scale_w")
+    scale_x, p_x = _vector_f32(scale_x, n, "scale_x")
+    bias, p_b = _vector_f32(bias, m, "bias")
+    c = x.new_empty((n, m), dtype=out_dtype or torch.bfloat16)
+    d = ScaledDesc(code, out, m, n, k, a_c.data_ptr(), lda, meta_tc.data_ptr(), x.data_ptr(), ldx,
+                   p_w, p_x, p_b, c.data_ptr(), 0, 0)
+    _check(lib.sp24_gemm_scaled(ctypes.byref(d), s), "sp24_gemm_scaled")
+    return c
 
 
 def gemm_scaled(a_c, meta_tc, x, scale_w=None, scale_x=None, *, bias=None, out_dtype=None,
@@ -525,97 +544,71 @@ def gemm_scaled(a_c, meta_tc, x, scale_w=None, scale_x=None, *, bias=None, out_d
     (a_c [m, k/2] of the same type, tcgen05 metadata image) with a scale for
     each channel (scale_w [m]) and each token (scale_x [n]) -> [n, m] of
     out_dtype (bfloat16, float16 or float32; default bfloat16)."""
-    import torch
-    lib = load()
-    out_dtype = out_dtype or torch.bfloat16
-    codes = {torch.int8: I8, torch.float8_e4m3fn: E4M3}
-    outs = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
-    if x.dtype not in codes or a_c.dtype != x.dtype:
-        raise ValueError(f"gemm_scaled: {x.dtype} tokens and {a_c.dtype} weights; both int8 or "
-                         "both float8_e4m3fn are wanted")
-    if out_dtype not in outs:
-        raise ValueError(f"gemm_scaled: out_dtype {out_dtype}")
-    with _On(_same_device(a_c, meta_tc, x, scale_w, scale_x, bias), stream) as s:
-        a_c = _tma_rows(a_c, "a_c")
-        m, k = a_c.shape[0], 2 * a_c.shape[1]
-        x = _tma_rows(x, "x", k)
-        n = x.shape[0]
-        if meta_tc.numel() * meta_tc.element_size() != meta_tc_bytes(m, k):
-            raise ValueError(f"meta_tc: {meta_tc.numel()} bytes, {meta_tc_bytes(m, k)} expected")
-        keep = []
-        for t, size, what in ((scale_w, m, "scale_w"), (scale_x, n, "scale_x"), (bias, m, "bias")):
-            if t is not None and (t.dtype != torch.float32 or t.numel() != size):
-                raise ValueError(f"{what}: {size} float32 values are wanted")
-            keep.append(t if t is None else t.contiguous())
-        c = torch.empty((n, m), dtype=out_dtype, device=x.device)
-        d = ScaledDesc()
-        d.dtype, d.cdtype, d.m, d.n, d.k = codes[x.dtype], outs[out_dtype], m, n, k
-        d.a_c, d.lda_c, d.meta = _ptr(a_c), _tma_ld(a_c), _ptr(meta_tc)
-        d.x, d.ldx = _ptr(x), _tma_ld(x)
-        d.scale_m, d.scale_n, d.bias = (_ptr(t) for t in keep)
-        d.c = _ptr(c)
-        _check(lib.sp24_gemm_scaled(ctypes.byref(d), s), "sp24_gemm_scaled")
-    return c
+    return _on(_same_device(x, a_c, meta_tc, scale_w, scale_x, bias), stream, _gemm_scaled, a_c,
+               meta_tc, x, scale_w, scale_x, bias, out_dtype)
 
 
-def _ffn_desc(x, w_gate, w_up, act):
-    import torch
-    if x.dtype not in (torch.float16, torch.bfloat16) or {w_gate.dtype, w_up.dtype} != {x.dtype}:
+def _ffn_desc(x, w_gate, w_up, act, saved=None):
+    """(descriptor, tensors it points to)."""
+    dt = (_codes or _code_tables())["16"].get(x.dtype)
+    if dt is None or w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
         raise ValueError(f"ffn_gated: {x.dtype}, {w_gate.dtype}, {w_up.dtype}; one of float16 and "
                          "bfloat16 for all is wanted")
-    x = _tma_rows(x, "x")
-    w_gate = _tma_rows(w_gate, "w_gate", x.shape[1])
-    w_up = _tma_rows(w_up, "w_up", x.shape[1], w_gate.shape[0])
-    d = FfnDesc()
-    d.dtype, d.act = dtype_code(x.dtype), act
-    d.t, d.h, d.f = x.shape[0], x.shape[1], w_gate.shape[0]
-    d.x, d.ldx = _ptr(x), _tma_ld(x)
-    d.w_gate, d.ld_gate, d.w_up, d.ld_up = _ptr(w_gate), _tma_ld(w_gate), _ptr(w_up), _tma_ld(w_up)
+    x, ldx = _tma_rows(x, "x")
+    t, h = x.shape
+    w_gate, ldg = _tma_rows(w_gate, "w_gate", h)
+    f = w_gate.shape[0]
+    w_up, ldu = _tma_rows(w_up, "w_up", h, f)
+    p_saved, n_saved = (0, 0) if saved is None else (saved.data_ptr(), saved.nbytes)
+    d = FfnDesc(dt, t, h, f, act, x.data_ptr(), ldx, w_gate.data_ptr(), ldg, w_up.data_ptr(), ldu,
+                p_saved, n_saved, 0)
     return d, (x, w_gate, w_up)
+
+
+def _ffn_forward(s, x, w_gate, w_up, act, save):
+    import torch
+    lib = _lib or load()
+    d, keep = _ffn_desc(x, w_gate, w_up, act)
+    out = x.new_empty((d.t, d.f))
+    if save:
+        saved = x.new_empty((lib.sp24_ffn_saved_bytes(d.t, d.f),), dtype=torch.uint8)
+        d.saved, d.saved_bytes = saved.data_ptr(), saved.nbytes
+    _check(lib.sp24_ffn_forward(ctypes.byref(d), out.data_ptr(), 0, s), "sp24_ffn_forward")
+    del keep
+    return (out, saved) if save else out
 
 
 def ffn_gated(x, w_gate, w_up, *, act=ACT_SILU, save=False, stream=None):
     """sp24_ffn_forward: act(x w_gate^T) * (x w_up^T) -> [t, f]; with save=True
     also the opaque buffer that ffn_gated_backward takes."""
+    return _on(_same_device(x, w_gate, w_up), stream, _ffn_forward, x, w_gate, w_up, act, save)
+
+
+def _ffn_backward(s, d_out, x, w_gate, w_up, saved, act, need_dx, need_dw):
     import torch
-    lib = load()
-    with _On(_same_device(x, w_gate, w_up), stream) as s:
-        d, keep = _ffn_desc(x, w_gate, w_up, act)
-        out = torch.empty((d.t, d.f), dtype=x.dtype, device=x.device)
-        saved = None
-        if save:
-            saved = torch.empty(lib.sp24_ffn_saved_bytes(d.t, d.f), dtype=torch.uint8,
-                                device=x.device)
-            d.saved, d.saved_bytes = _ptr(saved), saved.numel()
-        _check(lib.sp24_ffn_forward(ctypes.byref(d), _ptr(out), 0, s), "sp24_ffn_forward")
-        del keep
-    return (out, saved) if save else out
+    lib = _lib or load()
+    if d_out.dtype != x.dtype:
+        raise ValueError(f"ffn_gated_backward: {d_out.dtype} beside {x.dtype}")
+    d, keep = _ffn_desc(x, w_gate, w_up, act, saved)
+    d_out, ldd = _rows2d(d_out, "d_out", d.f, d.t)
+    dx = x.new_empty((d.t, d.h)) if need_dx else None
+    dw_gate = dw_up = None
+    if need_dw:
+        dw_gate, dw_up = x.new_empty((d.f, d.h)), x.new_empty((d.f, d.h))
+    ws = x.new_empty((lib.sp24_ffn_workspace_bytes(d.t, d.f),), dtype=torch.uint8)
+    g = FfnGrads(d_out.data_ptr(), ldd, _ptr(dx), 0, _ptr(dw_gate), 0, _ptr(dw_up), 0,
+                 ws.data_ptr(), ws.nbytes)
+    _check(lib.sp24_ffn_backward(ctypes.byref(d), ctypes.byref(g), s), "sp24_ffn_backward")
+    del keep
+    return dx, dw_gate, dw_up
 
 
 def ffn_gated_backward(d_out, x, w_gate, w_up, saved, *, act=ACT_SILU, need_dx=True,
                        need_dw=True, stream=None):
     """sp24_ffn_backward: (dx, dw_gate, dw_up) from dL/dout and what
     ffn_gated(save=True) kept (None for gradients that are not wanted)."""
-    import torch
-    lib = load()
-    if d_out.dtype != x.dtype:
-        raise ValueError(f"ffn_gated_backward: {d_out.dtype} beside {x.dtype}")
-    with _On(_same_device(d_out, x, w_gate, w_up, saved), stream) as s:
-        d, keep = _ffn_desc(x, w_gate, w_up, act)
-        d_out = _rows2d(d_out, "d_out", d.f, d.t)
-        d.saved, d.saved_bytes = _ptr(saved), saved.numel()
-        new = lambda *shape: torch.empty(shape, dtype=x.dtype, device=x.device)  # noqa: E731
-        dx = new(d.t, d.h) if need_dx else None
-        dw_gate, dw_up = (new(d.f, d.h), new(d.f, d.h)) if need_dw else (None, None)
-        ws = torch.empty(lib.sp24_ffn_workspace_bytes(d.t, d.f), dtype=torch.uint8,
-                         device=x.device)
-        g = FfnGrads()
-        g.d_out, g.ld_d_out = _ptr(d_out), _ld(d_out)
-        g.dx, g.dw_gate, g.dw_up = _ptr(dx), _ptr(dw_gate), _ptr(dw_up)
-        g.workspace, g.workspace_bytes = _ptr(ws), ws.numel()
-        _check(lib.sp24_ffn_backward(ctypes.byref(d), ctypes.byref(g), s), "sp24_ffn_backward")
-        del keep
-    return dx, dw_gate, dw_up
+    return _on(_same_device(x, d_out, w_gate, w_up, saved), stream, _ffn_backward, d_out, x,
+               w_gate, w_up, saved, act, need_dx, need_dw)
 
 
 def ipc_handle(t):
