@@ -40,7 +40,7 @@ LIB_DEPS = ["sp24_api.cu", "sp24_gemm_kernel.cuh", "sp24_gemm2sm_kernel.cuh",
 # Translation units of the library and the files each one reads.
 LIB_UNITS = {
     "sp24_api.cu": LIB_DEPS + [os.path.join("..", "dropin", "sp24_raw_kernel.cuh")],
-    "sp24_mlp.cu": ["sp24_mlp.cu", "sp24_host.cuh", "sp24_rows.cuh", "sp24_stream_kernel.cuh",
+    "sp24_mlp.cu": ["sp24_mlp.cu", "sp24_host.cuh", "sp24_rows.cuh", "sp24_stream_kernel.cuh", "sp24_scaled_pair_kernel.cuh",
                     "sp24_ffn_kernel.cuh", "sp24_gemm2sm_kernel.cuh", "sp24_gemm_kernel.cuh",
                     "sp24_gemm_splitk_kernel.cuh", "sp24_ptx.cuh"],
 }

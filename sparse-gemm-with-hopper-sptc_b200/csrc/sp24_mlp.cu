@@ -6,6 +6,7 @@
 #include "sp24_ffn_kernel.cuh"
 #include "sp24_host.cuh"
 #include "sp24_rows.cuh"
+#include "sp24_scaled_pair_kernel.cuh"
 #include "sp24_stream_kernel.cuh"
 
 using namespace sp24host;
@@ -249,14 +250,19 @@ sp24_status launch_stream(const FfnCall& c, const CUtensorMap& a, const CUtensor
   }
 }
 
-template <int OP>
-sp24_status scaled(const FfnCall& c, const sp24_scaled_desc* d) {
+// Tensor map of 8-bit rows in boxes of 128 columns.
+sp24_status encode_8(CUtensorMap* map, const void* base, int rows, int cols, int64_t ld, int box_rows) {
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, static_cast<uint64_t>(cols),
+                   static_cast<uint64_t>(rows), static_cast<uint64_t>(ld), 128,
+                   static_cast<uint32_t>(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+inline int out_type(const sp24_scaled_desc* d) { return d->cdtype == SP24_F32 ? 2 : static_cast<int>(d->cdtype); }
+inline int static_weights() { return (sp24_get_launch_hints() & SP24_HINT_STATIC_WEIGHTS) != 0; }
+
+template <int I8>
+sp24_status scaled_few(const FfnCall& c, const sp24_scaled_desc* d) {
   CUtensorMap a, b;
-  auto encode_8 = [](CUtensorMap* map, const void* base, int rows, int cols, int64_t ld, int box_rows) {
-    return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, static_cast<uint64_t>(cols),
-                     static_cast<uint64_t>(rows), static_cast<uint64_t>(ld), 128,
-                     static_cast<uint32_t>(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
-  };
   sp24_status st = encode_8(&a, d->a_c, d->m, d->k / 2, stride_or(d->lda_c, d->k / 2), 128);
   if (st == SP24_OK) st = encode_8(&b, d->x, d->n, d->k, stride_or(d->ldx, d->k), stream_bn(d->n));
   if (st != SP24_OK) return st;
@@ -266,10 +272,47 @@ sp24_status scaled(const FfnCall& c, const sp24_scaled_desc* d) {
   p.meta = d->meta;
   p.meta_mblocks = meta_mblocks(d->m), p.katoms = meta_katoms(d->k);
   p.scale_m = d->scale_m, p.scale_n = d->scale_n, p.bias = d->bias;
-  p.out = d->c, p.ldo = stride_or(d->ldc, d->m);
-  p.out_type = d->cdtype == SP24_F32 ? 2 : static_cast<int>(d->cdtype);
-  p.static_weights = (sp24_get_launch_hints() & SP24_HINT_STATIC_WEIGHTS) != 0;
-  return launch_stream<OP>(c, a, a, b, p);
+  p.out = d->c, p.ldo = stride_or(d->ldc, d->m), p.out_type = out_type(d);
+  p.static_weights = static_weights();
+  return launch_stream<I8 ? sp24::kStreamI8 : sp24::kStreamE4M3>(c, a, a, b, p);
+}
+
+template <int I8, int MB, int BN>
+sp24_status scaled_pair(const FfnCall& c, const sp24_scaled_desc* d) {
+  using C = sp24::ScaledPairCfg<I8, MB, BN>;
+  auto kern = sp24::scaled_pair_kernel<I8, MB, BN>;
+  static std::atomic<bool> attr_set[kMaxDevices];
+  sp24_status st = ensure_kernel_attrs(kern, attr_set, C::SMEM_BYTES);
+  if (st != SP24_OK) return st;
+  CUtensorMap a, b, e;
+  const int mblocks = meta_mblocks(d->m), katoms = meta_katoms(d->k);
+  st = encode_8(&a, d->a_c, d->m, d->k / 2, stride_or(d->lda_c, d->k / 2), 128);
+  if (st == SP24_OK) st = encode_8(&b, d->x, d->n, d->k, stride_or(d->ldx, d->k), C::HALF);
+  if (st == SP24_OK)
+    st = encode_2d(&e, CU_TENSOR_MAP_DATA_TYPE_UINT8, d->meta, 256,
+                   static_cast<uint64_t>(katoms) * mblocks * 8, 256, 256, 8, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (st != SP24_OK) return st;
+  sp24::ScaledPairParams p{};
+  p.m = d->m, p.n = d->n, p.k = d->k;
+  p.m_tiles = (d->m + MB * 256 - 1) / (MB * 256), p.n_tiles = (d->n + BN - 1) / BN;
+  p.k_stages = (d->k + C::BKD - 1) / C::BKD;
+  p.group_m = 8;
+  p.meta_mblocks = mblocks;
+  p.scale_m = d->scale_m, p.scale_n = d->scale_n, p.bias = d->bias;
+  p.out = d->c, p.ldo = stride_or(d->ldc, d->m), p.out_type = out_type(d);
+  p.static_weights = static_weights();
+  p.status = c.status;
+  p.timeout_ns = kDefaultTimeoutNs;
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  if (tiles > 0x7fffffff / 2) return SP24_ERR_SHAPE;
+  const unsigned pairs = static_cast<unsigned>(std::min<long long>(tiles, c.sm_count / 2));
+  return launch_gemm_kernel(kern, 2 * pairs, sp24::kPairThreads, C::SMEM_BYTES, c.stream, 0, true, a, b, e, p);
+}
+
+template <int I8>
+sp24_status scaled(const FfnCall& c, const sp24_scaled_desc* d) {
+  if (d->n <= kStreamMaxTokens) return scaled_few<I8>(c, d);
+  return scaled_pair<I8, 2, 224>(c, d);
 }
 
 template <int DT>
@@ -285,7 +328,7 @@ sp24_status ffn_forward_few(const FfnCall& c, const sp24_ffn_desc* d, void* out,
   p.out = out, p.ldo = ld_out, p.out_type = DT;
   p.saved = static_cast<float*>(d->saved), p.ld_saved = ffn_ld(d->f);
   p.silu = d->act == SP24_ACT_SILU;
-  p.static_weights = (sp24_get_launch_hints() & SP24_HINT_STATIC_WEIGHTS) != 0;
+  p.static_weights = static_weights();
   return launch_stream<DT == 0 ? sp24::kStreamF16 : sp24::kStreamBF16>(c, a, a2, b, p);
 }
 
@@ -381,7 +424,7 @@ sp24_status sp24_gemm_scaled(const sp24_scaled_desc* d, sp24_stream_t stream) {
   st = device_info(&di);
   if (st != SP24_OK) return st;
   const FfnCall c{di->sm_count, d->status_dev ? d->status_dev : di->status_word, as_stream(stream)};
-  return d->dtype == SP24_I8 ? scaled<sp24::kStreamI8>(c, d) : scaled<sp24::kStreamE4M3>(c, d);
+  return d->dtype == SP24_I8 ? scaled<1>(c, d) : scaled<0>(c, d);
 }
 
 size_t sp24_ffn_saved_bytes(int t, int f) {

@@ -1,0 +1,329 @@
+// sp24_scaled_pair_kernel.cuh — the 8-bit 2:4 product with channel and token
+// scales on CTA pairs, for many tokens.
+//
+//   acc[r][t] = sum_k W[r][k] x[t][k]        tcgen05.mma.sp.cta_group::2, M = 256,
+//   c[t][r]   = acc * scale_m[r] * scale_n[t] + bias[r]    N = BN, K = 64 per MMA
+//
+// What bounds it is the rate at which an SM can take operands in (about 64
+// bytes a clock, profiles/sp24_feed_probe.md), not the tensor pipe: a 256 x 256
+// tile takes 104 bytes per clock of sparse 8-bit MMAs.  Compressed weights are the
+// cheaper operand (half the values, plus an eighth for the codes), so a pair
+// computes MB = 2 blocks of 256 weight rows against one staged block of
+// BN = 224 tokens: 68 KB per 896 clocks, 78 bytes a clock.  The two
+// accumulators take 2 x 224 TMEM columns and the double-buffered metadata the
+// remaining 2 x 16; the accumulators are therefore single-buffered, and the
+// epilogue hands each back as soon as its columns are in registers.
+//
+// Accumulator lanes are weight rows, i.e. neighbouring features of a token's
+// output row: a warp's store of one token is one contiguous 64-byte run.
+//
+// Roles per CTA (11 warps), as in sp24_gemm2sm_kernel.cuh: warp 0 loads weights
+// and metadata, warp 10 tokens, warp 1 of the leader issues, warps 2-9 drain.
+#pragma once
+
+#include "sp24_gemm2sm_kernel.cuh"
+#include "sp24_ptx.cuh"
+#include "sp24_stream_kernel.cuh"
+
+namespace sp24 {
+
+struct ScaledPairParams {
+  int m, n, k;
+  int m_tiles, n_tiles, k_stages;
+  int group_m;
+  int meta_mblocks;
+  const float *scale_m, *scale_n, *bias;
+  void* out;
+  long long ldo;
+  int out_type;
+  int static_weights;
+  int* status;
+  unsigned long long timeout_ns;
+};
+
+template <int I8, int MB, int BN>
+struct ScaledPairCfg {
+  static constexpr int BKD = 256;                       // dense K per stage
+  static constexpr int MMAS = 4;
+  static constexpr int A_BOX = kBlockM * 128;
+  static constexpr int A_BYTES = MB * A_BOX;
+  static constexpr int HALF = BN / 2;                   // tokens staged per CTA
+  static constexpr int B_BOX = HALF * 128;
+  static constexpr int B_BYTES = 2 * B_BOX;
+  static constexpr int E_BYTES = MB * 2 * kAtomBytes;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + E_BYTES;
+  static constexpr int STAGES_RAW = (kSmemBudget - 1024) / STAGE_BYTES;
+  static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
+  // TMEM: accumulator b at column 256 b, metadata buffer e after accumulator e.
+  static constexpr int E_COL = BN;
+  static constexpr uint32_t IDESC =
+      I8 ? ((1u << 2) | (2u << 4) | (1u << 7) | (1u << 10) | ((BN >> 3) << 17) | ((256u >> 4) << 24))
+         : make_idesc_sparse(0, BN, 256, false);
+  static constexpr int CW = BN / 2;                     // columns per epilogue warp
+  static_assert(BN % 32 == 0 && BN + MB * 8 <= 256, "tokens per tile");
+  static_assert(B_BOX % 1024 == 0 && STAGE_BYTES % 1024 == 0, "boxes stay 1024-aligned");
+  static_assert(STAGES >= 3, "ring");
+};
+
+SP24_DEV void tc_mma_sp_pair_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t e, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.sp.cta_group::2.kind::i8 [%0], %1, %2, [%3], %4, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(e), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+SP24_DEV void scaled_tile(const ScaledPairParams& P, int t, int& mt, int& nt) {
+  const int per_group = P.group_m * P.n_tiles;
+  const int g = t / per_group;
+  const int first = g * P.group_m;
+  const int gm = min(P.m_tiles - first, P.group_m);
+  const int r = t - g * per_group;
+  mt = first + r % gm;
+  nt = r / gm;
+}
+
+// tmA: a_c, tmB: tokens, tmE: the metadata image as rows of 256 bytes (8 to an atom).
+template <int I8, int MB, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    scaled_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                       const __grid_constant__ CUtensorMap tmE, const ScaledPairParams P) {
+#if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
+  using C = ScaledPairCfg<I8, MB, BN>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t accf_bar;
+  __shared__ __align__(8) uint64_t acce_bar[MB];
+  __shared__ __align__(8) uint64_t drain_bar;
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ volatile int abort_sh;
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int prank = static_cast<int>(cluster_ctarank());
+  const bool leader = prank == 0;
+  const int pair = static_cast<int>(blockIdx.x >> 1);
+  const int npairs = static_cast<int>(gridDim.x >> 1);
+  const int num_tiles = P.m_tiles * P.n_tiles;
+  const uint64_t tmo = P.timeout_ns;
+
+  if (threadIdx.x == 0) {
+    abort_sh = 0;
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&accf_bar, 1);
+    for (int b = 0; b < MB; ++b) mbar_init(&acce_bar[b], 2 * kPairEpiWarps);
+    mbar_init(&drain_bar, 1);
+    fence_barrier_init();
+    // Armed here for the first use, by the MMA warp for later ones; both CTAs'
+    // bytes land on the leader's barriers (TMA counts zero-filled ones too).
+    if (leader)
+      for (int s = 0; s < C::STAGES; ++s) mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmE);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&tmem_base_sh, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_sh;
+  griddep_launch_dependents();
+
+  if (warp == 0 || warp == kPairBWarp) {
+    // ------------------------------------------------------------ producers
+    // Warp 0: lanes 0 .. MB-1 a block of 128 a_c rows each, then an atom a lane;
+    // warp 10: the two 128-byte halves of the stage's tokens.
+    const bool is_b = warp == kPairBWarp;
+    if (is_b || !P.static_weights) griddep_wait();
+    const bool is_a = !is_b && lane < MB;
+    const int el = lane - MB;                           // block el / 2, atom el % 2
+    const int lanes = is_b ? 2 : 3 * MB;
+    const CUtensorMap* map = is_b ? &tmB : is_a ? &tmA : &tmE;
+    const uint32_t off = is_b   ? C::A_BYTES + lane * C::B_BOX
+                         : is_a ? lane * C::A_BOX
+                                : C::A_BYTES + C::B_BYTES + el * kAtomBytes;
+    const int dx = is_b ? C::BKD : is_a ? C::BKD / 2 : 0;
+    const int dy = is_b || is_a ? 0 : 2 * P.meta_mblocks * 8;
+    const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    uint32_t used_mask = 0, used_ph = 0;
+    for (int t = pair; t < num_tiles && ok; t += npairs) {
+      int mt, nt;
+      scaled_tile(P, t, mt, nt);
+      int x = is_b ? lane * 128 : 0, y;
+      if (is_b) {
+        y = nt * BN + prank * C::HALF;
+      } else if (is_a) {
+        y = (mt * MB + lane) * 256 + prank * 128;
+      } else {
+        // Blocks past the image belong to rows past m: any valid codes serve.
+        const int mb = min((mt * MB + (el >> 1)) * 2 + prank, P.meta_mblocks - 1);
+        y = ((el & 1) * P.meta_mblocks + mb) * 8;
+      }
+      for (int ks = 0; ks < P.k_stages; ++ks) {
+        int good = 1;
+        if (lane == 0) good = mbar_wait_fast(&empty_bar[s], ph ^ 1u, &abort_sh, tmo) ? 1 : 0;
+        if (__shfl_sync(0xffffffffu, good, 0) == 0) {
+          ok = false;
+          break;
+        }
+        if (leader && lane == 0) {
+          used_mask |= 1u << s;
+          used_ph = (used_ph & ~(1u << s)) | (ph << s);
+        }
+        if (lane < lanes)
+          tma_load_2d_pair(smem + s * C::STAGE_BYTES + off, map, full0 + s * sizeof(uint64_t), x, y);
+        x += dx;
+        y += dy;
+        if (++s == C::STAGES) s = 0, ph ^= 1u;
+      }
+    }
+    if (!ok && leader && lane == 0) {
+      // Error path: copies in flight land before the CTA leaves.
+      volatile int dummy = 0;
+      for (int i = 0; i < C::STAGES; ++i)
+        if (used_mask & (1u << i)) mbar_wait(&full_bar[i], (used_ph >> i) & 1u, &dummy, tmo);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader)
+    if (leader) {
+      const uint32_t base = smem_u32(smem);
+      const uint64_t adesc0 = make_sdesc(base, 16, 1024, kLayoutSW128);
+      const uint64_t bdesc0 = make_sdesc(base + C::A_BYTES, 16, 1024, kLayoutSW128);
+      const uint64_t edesc0 = make_sdesc(base + C::A_BYTES + C::B_BYTES, kAtomBytes, 128, kLayoutNone);
+      int s = 0;
+      uint32_t ph = 0, aph = 0, ebuf = 0;
+      bool ok = true, any = false;
+      for (int t = pair; t < num_tiles && ok; t += npairs) {
+        int mt, nt;
+        scaled_tile(P, t, mt, nt);
+        for (int ks = 0; ks < P.k_stages && ok; ++ks) {
+          if (!mbar_wait_warp(&full_bar[s], ph, &abort_sh, tmo)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
+          tc_fence_after();
+          ebuf ^= 1u;
+          const uint32_t e = tmem_base + ebuf * 256 + C::E_COL;
+          const int kleft = P.k - ks * C::BKD;
+          const uint64_t so = static_cast<uint64_t>(s * (C::STAGE_BYTES >> 4));
+          if (elect_one()) {
+#pragma unroll
+            for (int a = 0; a < MB * 2; ++a) tc_cp<2>(e + 4 * a, edesc0 + so + a * (kAtomBytes >> 4));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int b = 0; b < MB; ++b) {
+            if (ks == 0) {   // this accumulator's columns of the last tile are in registers
+              if (!mbar_wait_warp<true>(&acce_bar[b], aph ^ 1u, &abort_sh, tmo)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+            }
+            if (elect_one()) {
+#pragma unroll
+              for (int j = 0; j < C::MMAS; ++j)
+                if (j * 64 < kleft) {   // past K there is no metadata
+                  const uint64_t ad = adesc0 + so + b * (C::A_BOX >> 4) + j * 2;
+                  const uint64_t bd = bdesc0 + so + (j >> 1) * (C::B_BOX >> 4) + (j & 1) * 4;
+                  const uint32_t d = tmem_base + b * 256, ec = e + b * 8 + j * 2;
+                  const uint32_t acc = (ks > 0 || j > 0) ? 1u : 0u;
+                  if constexpr (I8) tc_mma_sp_pair_i8(d, ad, bd, ec, C::IDESC, acc);
+                  else tc_mma_sp_pair<1>(d, ad, bd, ec, C::IDESC, acc);
+                }
+            }
+            __syncwarp();
+            any = true;
+          }
+          if (!ok) break;
+          if (elect_one()) tc_commit_pair(&empty_bar[s], 3);
+          __syncwarp();
+          if (++s == C::STAGES) s = 0, ph ^= 1u;
+        }
+        if (!ok) break;
+        if (elect_one()) tc_commit_pair(&accf_bar, 3);
+        __syncwarp();
+        aph ^= 1u;
+      }
+      if (!ok && any) {
+        volatile int dummy = 0;
+        if (elect_one()) tc_commit_pair(&drain_bar, 1);
+        __syncwarp();
+        if (lane == 0) mbar_wait(&drain_bar, 0, &dummy, tmo);
+        __syncwarp();
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;
+    const int half = (warp - 2) >> 2;
+    const uint32_t acce0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
+    uint32_t aph = 0;
+    griddep_wait();   // scales and bias may come from the previous kernel
+    for (int t = pair; t < num_tiles; t += npairs) {
+      int mt, nt;
+      scaled_tile(P, t, mt, nt);
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait_sleepy(&accf_bar, aph, &abort_sh, tmo);
+      if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) == 0) break;
+      tc_fence_after();
+      aph ^= 1u;
+#pragma unroll 1
+      for (int b = 0; b < MB; ++b) {
+        uint32_t r[C::CW];
+        const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                            static_cast<uint32_t>(b * 256 + half * C::CW);
+#pragma unroll
+        for (int c = 0; c < C::CW; c += 16)
+          tmem_ld_x16(tb + c, *reinterpret_cast<uint32_t(*)[16]>(&r[c]));
+        tmem_ld_wait(r);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(acce0 + b * sizeof(uint64_t));
+        const int row = (mt * MB + b) * 256 + prank * 128 + q * 32 + lane;
+        const int t0 = nt * BN + half * C::CW;
+        if (row < P.m) {
+          const float sm = P.scale_m != nullptr ? P.scale_m[row] : 1.0f;
+          const float bias = P.bias != nullptr ? P.bias[row] : 0.0f;
+#pragma unroll
+          for (int j = 0; j < C::CW; ++j) {
+            if (t0 + j < P.n) {
+              const float sn = P.scale_n != nullptr ? __ldg(P.scale_n + t0 + j) : 1.0f;
+              const float a = I8 ? static_cast<float>(static_cast<int>(r[j])) : __uint_as_float(r[j]);
+              store_out(P.out, P.out_type, (t0 + j) * P.ldo + row, fmaf(a, sm * sn, bias));
+            }
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+  if (threadIdx.x == 0 && abort_sh != 0 && P.status != nullptr) atomicExch(P.status, 1);
+#endif
+}
+
+}  // namespace sp24
