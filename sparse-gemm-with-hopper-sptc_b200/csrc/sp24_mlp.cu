@@ -300,6 +300,7 @@ sp24_status scaled_pair(const FfnCall& c, const sp24_scaled_desc* d) {
   p.meta_mblocks = mblocks;
   p.scale_m = d->scale_m, p.scale_n = d->scale_n, p.bias = d->bias;
   p.out = d->c, p.ldo = stride_or(d->ldc, d->m), p.out_type = out_type(d);
+  p.words = reinterpret_cast<uintptr_t>(d->c) % 4 == 0 && p.ldo % 2 == 0;
   p.static_weights = static_weights();
   p.status = c.status;
   p.timeout_ns = kDefaultTimeoutNs;

@@ -36,6 +36,7 @@ struct ScaledPairParams {
   void* out;
   long long ldo;
   int out_type;
+  int words;          // 16-bit output rows start on 4-byte boundaries
   int static_weights;
   int* status;
   unsigned long long timeout_ns;
@@ -85,6 +86,45 @@ SP24_DEV void scaled_tile(const ScaledPairParams& P, int t, int& mt, int& nt) {
   nt = r / gm;
 }
 
+// Warp-collective: CW accumulator columns (tokens t0 ..) of 32 weight rows, lane
+// l holding row `row` = row0 + l, scaled and stored.  sn: the tokens' scales in
+// shared memory.  16-bit outputs leave as whole words: neighbouring lanes swap
+// halves, so that even lanes store two rows of one token and odd lanes of the
+// next (paired: rows start on words, all tokens and rows present).
+template <int I8, int CW, int OUT>
+SP24_DEV void scaled_emit(const ScaledPairParams& P, const uint32_t (&r)[CW], int row, int t0, const float* sn,
+                          bool paired) {
+  const int lane = threadIdx.x & 31;
+  const bool live = row < P.m;
+  const float sm = live && P.scale_m != nullptr ? P.scale_m[row] : 1.0f;
+  const float bias = live && P.bias != nullptr ? P.bias[row] : 0.0f;
+  auto value = [&](int j) {
+    const float a = I8 ? static_cast<float>(static_cast<int>(r[j])) : __uint_as_float(r[j]);
+    return fmaf(a, sm * sn[j], bias);
+  };
+  if constexpr (OUT != 2) {
+    if (paired) {
+      const bool odd = lane & 1;
+      uint16_t* p = static_cast<uint16_t*>(P.out) + (t0 + odd) * P.ldo + (row - odd);
+#pragma unroll
+      for (int j = 0; j < CW; j += 2) {
+        const uint32_t mine = pack16<OUT>(value(j), value(j + 1));
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+        *reinterpret_cast<uint32_t*>(p) = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+        p += 2 * P.ldo;
+      }
+      return;
+    }
+  }
+  if (!live) return;
+  long long o = t0 * P.ldo + row;
+#pragma unroll
+  for (int j = 0; j < CW; ++j) {
+    if (t0 + j < P.n) store_out(P.out, OUT, o, value(j));
+    o += P.ldo;
+  }
+}
+
 // tmA: a_c, tmB: tokens, tmE: the metadata image as rows of 256 bytes (8 to an atom).
 template <int I8, int MB, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
@@ -98,6 +138,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   __shared__ __align__(8) uint64_t accf_bar;
   __shared__ __align__(8) uint64_t acce_bar[MB];
   __shared__ __align__(8) uint64_t drain_bar;
+  __shared__ float sn_sh[kPairEpiWarps][C::CW];   // each epilogue warp's token scales
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile int abort_sh;
 
@@ -280,11 +321,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     for (int t = pair; t < num_tiles; t += npairs) {
       int mt, nt;
       scaled_tile(P, t, mt, nt);
+      float* sn = sn_sh[warp - 2];
+      __syncwarp();
+      for (int j = lane; j < C::CW; j += 32) {
+        const int tok = nt * BN + half * C::CW + j;
+        sn[j] = P.scale_n != nullptr && tok < P.n ? P.scale_n[tok] : 1.0f;
+      }
+      __syncwarp();
       bool ok = true;
       if (lane == 0) ok = mbar_wait_sleepy(&accf_bar, aph, &abort_sh, tmo);
       if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) == 0) break;
       tc_fence_after();
       aph ^= 1u;
+      const int t0 = nt * BN + half * C::CW;
 #pragma unroll 1
       for (int b = 0; b < MB; ++b) {
         uint32_t r[C::CW];
@@ -298,19 +347,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(acce0 + b * sizeof(uint64_t));
         const int row = (mt * MB + b) * 256 + prank * 128 + q * 32 + lane;
-        const int t0 = nt * BN + half * C::CW;
-        if (row < P.m) {
-          const float sm = P.scale_m != nullptr ? P.scale_m[row] : 1.0f;
-          const float bias = P.bias != nullptr ? P.bias[row] : 0.0f;
-#pragma unroll
-          for (int j = 0; j < C::CW; ++j) {
-            if (t0 + j < P.n) {
-              const float sn = P.scale_n != nullptr ? __ldg(P.scale_n + t0 + j) : 1.0f;
-              const float a = I8 ? static_cast<float>(static_cast<int>(r[j])) : __uint_as_float(r[j]);
-              store_out(P.out, P.out_type, (t0 + j) * P.ldo + row, fmaf(a, sm * sn, bias));
-            }
-          }
-        }
+        const bool paired = P.words && t0 + C::CW <= P.n && row - lane + 32 <= P.m;
+        if (P.out_type == 2) scaled_emit<I8, C::CW, 2>(P, r, row, t0, sn, paired);
+        else if (P.out_type == 1) scaled_emit<I8, C::CW, 1>(P, r, row, t0, sn, paired);
+        else scaled_emit<I8, C::CW, 0>(P, r, row, t0, sn, paired);
       }
     }
   }
