@@ -77,7 +77,7 @@ sp24_status launch_rows_kernel(const sp24::RowsParams& p, const DeviceInfo& di, 
   const int smem = V == 8 ? inputs * VPT * static_cast<int>(threads) * 16 : 0;
   const int t = static_cast<int>(threads);
   int blocks = std::min({2048 / t, 65536 / (regs.load(std::memory_order_relaxed) * t), 32});
-  if (smem > 0) blocks = std::min(blocks, kSmem / smem);
+  if (V == 8) blocks = std::min(blocks, kSmem / std::max(smem, 1));
   blocks = std::max(blocks, 1);
   const long long per_block = ONE_WARP ? t / 32 : 1;
   const long long want = (p.rows + per_block - 1) / per_block;
@@ -230,10 +230,15 @@ sp24_status launch_stream_bn(const FfnCall& c, const CUtensorMap& a, const CUten
   if (tiles * sp24::kStreamMaxSplits > 0x7fffffff) return SP24_ERR_SHAPE;
   p.splits = static_cast<int>(std::max(1LL, std::min<long long>({c.sm_count / tiles, sp24::kStreamMaxSplits,
                                                                  p.stages})));
+  // No more slots than a CTA has stages: what is left of the SM's shared memory
+  // lets the next kernel's CTAs start their prologue beside this one's tail
+  // (4096 x 4096, 1 token, back to back: 6.1 -> 5.6 us).
+  p.ring = std::min(C::STAGES, (p.stages + p.splits - 1) / p.splits);
+  const int smem = std::max(p.ring * C::STAGE_BYTES, p.splits > 1 ? C::PARKED : 0) + 1024;
   p.status = c.status;
   p.timeout_ns = kDefaultTimeoutNs;
   return launch_gemm_kernel(kern, static_cast<unsigned>(tiles * p.splits), sp24::kStreamThreads,
-                            C::SMEM_BYTES, c.stream, static_cast<unsigned>(p.splits), true, a, a2, b, p);
+                            static_cast<size_t>(smem), c.stream, static_cast<unsigned>(p.splits), true, a, a2, b, p);
 }
 
 // rows of a TMA box of B for n tokens
@@ -307,13 +312,28 @@ sp24_status scaled_pair(const FfnCall& c, const sp24_scaled_desc* d) {
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
   if (tiles > 0x7fffffff / 2) return SP24_ERR_SHAPE;
   const unsigned pairs = static_cast<unsigned>(std::min<long long>(tiles, c.sm_count / 2));
-  return launch_gemm_kernel(kern, 2 * pairs, sp24::kPairThreads, C::SMEM_BYTES, c.stream, 0, true, a, b, e, p);
+  return launch_gemm_kernel(kern, 2 * pairs, sp24::kScaledThreads, C::SMEM_BYTES, c.stream, 0, true, a, b, e, p);
 }
 
+// Which kernel.  Up to 32 tokens the weights' bytes decide, and the streaming
+// kernel splits K over as many SMs as there are.  From 33 to 128 tokens a pair
+// that stages half the tokens per SM wins where 256-row tiles alone occupy
+// three quarters of the pairs (14336 x 4096, 64 / 128 tokens: 13.7 / 13.9 us
+// against 15.0 / 21.8; 4096 x 14336 has 16 such tiles: 28 us against 13 / 17).
+// Beyond, tiles of one 256-row block x 128 tokens fill few waves, and tiles of
+// two blocks x 224 tokens load less per product: one wave of the large tile
+// costs 2.6 of the small one (K = 4096: 17.5 and 6.7 us), so it is taken where
+// it saves more waves than that (14336 x 4096: 200 tokens 26.3 against 20.1 us
+// on the small tile, 1024 tokens 41.6 against 55.0).
 template <int I8>
 sp24_status scaled(const FfnCall& c, const sp24_scaled_desc* d) {
-  if (d->n <= kStreamMaxTokens) return scaled_few<I8>(c, d);
-  return scaled_pair<I8, 2, 224>(c, d);
+  const long long pairs = c.sm_count / 2;
+  const long long blocks = (d->m + 255) / 256;
+  if (d->n <= 32 || (d->n <= kStreamMaxTokens && 4 * blocks < 3 * pairs)) return scaled_few<I8>(c, d);
+  auto waves = [&](long long tiles) { return (tiles + pairs - 1) / pairs; };
+  const long long small = waves(blocks * ((d->n + 127) / 128));
+  const long long large = waves((d->m + 511LL) / 512 * ((d->n + 223LL) / 224));
+  return 10 * small > 26 * large ? scaled_pair<I8, 2, 224>(c, d) : scaled_pair<I8, 1, 128>(c, d);
 }
 
 template <int DT>

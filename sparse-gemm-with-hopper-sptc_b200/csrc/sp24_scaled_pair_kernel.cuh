@@ -4,21 +4,30 @@
 //   acc[r][t] = sum_k W[r][k] x[t][k]        tcgen05.mma.sp.cta_group::2, M = 256,
 //   c[t][r]   = acc * scale_m[r] * scale_n[t] + bias[r]    N = BN, K = 64 per MMA
 //
-// What bounds it is the rate at which an SM can take operands in (about 64
-// bytes a clock, profiles/sp24_feed_probe.md), not the tensor pipe: a 256 x 256
-// tile takes 104 bytes per clock of sparse 8-bit MMAs.  Compressed weights are the
-// cheaper operand (half the values, plus an eighth for the codes), so a pair
-// computes MB = 2 blocks of 256 weight rows against one staged block of
-// BN = 224 tokens: 68 KB per 896 clocks, 78 bytes a clock.  The two
-// accumulators take 2 x 224 TMEM columns and the double-buffered metadata the
-// remaining 2 x 16; the accumulators are therefore single-buffered, and the
-// epilogue hands each back as soon as its columns are in registers.
+// Two tiles.  The tensor pipe takes about 11.6k multiply-adds a clock and SM of
+// this kind, an SM takes in about 64 bytes a clock (profiles/sp24_feed_probe.md),
+// and compressed weights are the cheaper operand (half the values, plus an eighth
+// for the codes).
+//   MB = 2, BN = 224  two blocks of 256 weight rows against one staged block of
+//                     tokens: 68 KB per 1273 clocks of MMAs and 256 of K.  The
+//                     accumulators take 2 x 224 TMEM columns and the
+//                     double-buffered metadata 2 x 16 of the rest, so they are
+//                     single-buffered; the epilogue hands each back once its
+//                     columns are in registers.
+//   MB = 1, BN = 128  36 KB per 364 clocks: more loading per product, but twice
+//                     as many tiles in both directions and two accumulator
+//                     buffers, for calls that do not fill the GPU with the other.
+// 14336 x 4096 int8, 4096 tokens (481 dense-equivalent GFLOP): 143 us, of which the
+// MMAs alone would take about 96 at the 1.7 GHz the power cap leaves; without its
+// stores the kernel takes 115, without its MMAs 114.  The layout of the stores
+// does not matter (full 128-byte lines: 144), nor do 128-deep stages in a ring
+// twice as long (their 64-byte weight rows load slower: 188).
 //
 // Accumulator lanes are weight rows, i.e. neighbouring features of a token's
 // output row: a warp's store of one token is one contiguous 64-byte run.
 //
-// Roles per CTA (11 warps), as in sp24_gemm2sm_kernel.cuh: warp 0 loads weights
-// and metadata, warp 10 tokens, warp 1 of the leader issues, warps 2-9 drain.
+// Roles per CTA: warps 0-7 drain the accumulators, warp 8 loads weights and
+// metadata, warp 10 the tokens, warp 9 of the leader issues the MMAs.
 #pragma once
 
 #include "sp24_gemm2sm_kernel.cuh"
@@ -26,6 +35,9 @@
 #include "sp24_stream_kernel.cuh"
 
 namespace sp24 {
+
+constexpr int kScaledThreads = 352;   // 11 warps: 0-7 epilogue, then one role each
+constexpr int kScaledAWarp = 8, kScaledMmaWarp = 9, kScaledBWarp = 10;
 
 struct ScaledPairParams {
   int m, n, k;
@@ -44,16 +56,18 @@ struct ScaledPairParams {
 
 template <int I8, int MB, int BN>
 struct ScaledPairCfg {
-  static constexpr int BKD = 256;                       // dense K per stage
-  static constexpr int MMAS = 4;
+  static constexpr int BKD = 256;                       // dense K per stage (rows of 128 bytes)
+  static constexpr int MMAS = BKD / 64;
   static constexpr int A_BOX = kBlockM * 128;
   static constexpr int A_BYTES = MB * A_BOX;
   static constexpr int HALF = BN / 2;                   // tokens staged per CTA
   static constexpr int B_BOX = HALF * 128;
-  static constexpr int B_BYTES = 2 * B_BOX;
-  static constexpr int E_BYTES = MB * 2 * kAtomBytes;
+  static constexpr int B_BOXES = BKD / 128;
+  static constexpr int B_BYTES = B_BOXES * B_BOX;
+  static constexpr int ATOMS = BKD / 128;               // per block
+  static constexpr int E_BYTES = MB * ATOMS * kAtomBytes;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + E_BYTES;
-  static constexpr int STAGES_RAW = (kSmemBudget - 1024) / STAGE_BYTES;
+  static constexpr int STAGES_RAW = (kSmemBudget - 5 * 1024) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
   // TMEM: accumulator b at column 256 b, metadata buffer e after accumulator e.
@@ -62,7 +76,7 @@ struct ScaledPairCfg {
       I8 ? ((1u << 2) | (2u << 4) | (1u << 7) | (1u << 10) | ((BN >> 3) << 17) | ((256u >> 4) << 24))
          : make_idesc_sparse(0, BN, 256, false);
   static constexpr int CW = BN / 2;                     // columns per epilogue warp
-  static_assert(BN % 32 == 0 && BN + MB * 8 <= 256, "tokens per tile");
+  static_assert(BN % 32 == 0 && BN + MB * ATOMS * 4 <= 256, "tokens per tile");
   static_assert(B_BOX % 1024 == 0 && STAGE_BYTES % 1024 == 0, "boxes stay 1024-aligned");
   static_assert(STAGES >= 3, "ring");
 };
@@ -86,48 +100,80 @@ SP24_DEV void scaled_tile(const ScaledPairParams& P, int t, int& mt, int& nt) {
   nt = r / gm;
 }
 
+// Two fp32 operations in one instruction.
+SP24_DEV float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+SP24_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
+template <int I8>
+SP24_DEV float sum_value(uint32_t a) {
+  return I8 ? static_cast<float>(static_cast<int>(a)) : __uint_as_float(a);
+}
+
 // Warp-collective: CW accumulator columns (tokens t0 ..) of 32 weight rows, lane
 // l holding row `row` = row0 + l, scaled and stored.  sn: the tokens' scales in
-// shared memory.  16-bit outputs leave as whole words: neighbouring lanes swap
-// halves, so that even lanes store two rows of one token and odd lanes of the
-// next (paired: rows start on words, all tokens and rows present).
+// shared memory.  The epilogue is bound by instruction issue (eight warps, two
+// blocks of 112 columns each), hence the paired arithmetic, and 16-bit outputs
+// leave as whole words: neighbouring lanes swap halves, so that even lanes store
+// two rows of one token and odd lanes of the next (words: rows start on words).
 template <int I8, int CW, int OUT>
-SP24_DEV void scaled_emit(const ScaledPairParams& P, const uint32_t (&r)[CW], int row, int t0, const float* sn,
-                          bool paired) {
+SP24_DEV void scaled_emit(const ScaledPairParams& P, const uint32_t (&r)[CW], int row, int t0, const float* sn) {
   const int lane = threadIdx.x & 31;
   const bool live = row < P.m;
-  const float sm = live && P.scale_m != nullptr ? P.scale_m[row] : 1.0f;
-  const float bias = live && P.bias != nullptr ? P.bias[row] : 0.0f;
-  auto value = [&](int j) {
-    const float a = I8 ? static_cast<float>(static_cast<int>(r[j])) : __uint_as_float(r[j]);
-    return fmaf(a, sm * sn[j], bias);
+  const float sm1 = live && P.scale_m != nullptr ? P.scale_m[row] : 1.0f;
+  const float b1 = live && P.bias != nullptr ? P.bias[row] : 0.0f;
+  const float2 sm = make_float2(sm1, sm1), bias = make_float2(b1, b1);
+  auto value2 = [&](int j) {
+    const float2 s = *reinterpret_cast<const float2*>(sn + j);
+    return fma2(make_float2(sum_value<I8>(r[j]), sum_value<I8>(r[j + 1])), mul2(sm, s), bias);
   };
-  if constexpr (OUT != 2) {
-    if (paired) {
-      const bool odd = lane & 1;
-      uint16_t* p = static_cast<uint16_t*>(P.out) + (t0 + odd) * P.ldo + (row - odd);
+  const int left = P.n - t0;   // tokens from t0 on
+  if constexpr (OUT == 2) {
+    if (!live) return;
+    float* p = static_cast<float*>(P.out) + t0 * P.ldo + row;
 #pragma unroll
-      for (int j = 0; j < CW; j += 2) {
-        const uint32_t mine = pack16<OUT>(value(j), value(j + 1));
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-        *reinterpret_cast<uint32_t*>(p) = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
-        p += 2 * P.ldo;
-      }
-      return;
+    for (int j = 0; j < CW; j += 2) {
+      const float2 v = value2(j);
+      if (j < left) p[0] = v.x;
+      if (j + 1 < left) p[P.ldo] = v.y;
+      p += 2 * P.ldo;
     }
-  }
-  if (!live) return;
-  long long o = t0 * P.ldo + row;
+  } else if (P.words && left >= CW && row - lane + 32 <= P.m) {
+    const int odd = lane & 1;
+    const uint32_t sel = odd ? 0x3276u : 0x5410u;
+    uint16_t* p = static_cast<uint16_t*>(P.out) + (t0 + odd) * P.ldo + (row - odd);
 #pragma unroll
-  for (int j = 0; j < CW; ++j) {
-    if (t0 + j < P.n) store_out(P.out, OUT, o, value(j));
-    o += P.ldo;
+    for (int j = 0; j < CW; j += 2) {
+      const float2 v = value2(j);
+      const uint32_t mine = pack16<OUT>(v.x, v.y);
+      *reinterpret_cast<uint32_t*>(p) = __byte_perm(mine, __shfl_xor_sync(0xffffffffu, mine, 1), sel);
+      p += 2 * P.ldo;
+    }
+  } else if (live) {
+    uint16_t* p = static_cast<uint16_t*>(P.out) + t0 * P.ldo + row;
+#pragma unroll
+    for (int j = 0; j < CW; j += 2) {
+      const float2 v = value2(j);
+      const uint32_t w = pack16<OUT>(v.x, v.y);
+      if (j < left) p[0] = static_cast<uint16_t>(w);
+      if (j + 1 < left) p[P.ldo] = static_cast<uint16_t>(w >> 16);
+      p += 2 * P.ldo;
+    }
   }
 }
 
 // tmA: a_c, tmB: tokens, tmE: the metadata image as rows of 256 bytes (8 to an atom).
 template <int I8, int MB, int BN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kScaledThreads, 1)
     scaled_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmE, const ScaledPairParams P) {
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
@@ -135,10 +181,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[C::STAGES];
   __shared__ __align__(8) uint64_t empty_bar[C::STAGES];
-  __shared__ __align__(8) uint64_t accf_bar;
-  __shared__ __align__(8) uint64_t acce_bar[MB];
+  __shared__ __align__(8) uint64_t accf_bar[2 / MB];
+  __shared__ __align__(8) uint64_t acce_bar[2];
   __shared__ __align__(8) uint64_t drain_bar;
-  __shared__ float sn_sh[kPairEpiWarps][C::CW];   // each epilogue warp's token scales
+  __shared__ __align__(16) float sn_sh[kPairEpiWarps][C::CW];   // each epilogue warp's token scales
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile int abort_sh;
 
@@ -159,8 +205,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
-    mbar_init(&accf_bar, 1);
-    for (int b = 0; b < MB; ++b) mbar_init(&acce_bar[b], 2 * kPairEpiWarps);
+    for (int b = 0; b < 2 / MB; ++b) mbar_init(&accf_bar[b], 1);
+    for (int b = 0; b < 2; ++b) mbar_init(&acce_bar[b], 2 * kPairEpiWarps);
     mbar_init(&drain_bar, 1);
     fence_barrier_init();
     // Armed here for the first use, by the MMA warp for later ones; both CTAs'
@@ -168,12 +214,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (leader)
       for (int s = 0; s < C::STAGES; ++s) mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
   }
-  if (warp == 0 && lane == 0) {
+  if (warp == kScaledAWarp && lane == 0) {
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
     tma_prefetch_desc(&tmE);
   }
-  if (warp == 1) {
+  if (warp == kScaledMmaWarp) {
     tmem_alloc_pair(&tmem_base_sh, 512);
     tmem_relinquish_pair();
   }
@@ -183,21 +229,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const uint32_t tmem_base = tmem_base_sh;
   griddep_launch_dependents();
 
-  if (warp == 0 || warp == kPairBWarp) {
+  if (warp == kScaledAWarp || warp == kScaledBWarp) {
     // ------------------------------------------------------------ producers
-    // Warp 0: lanes 0 .. MB-1 a block of 128 a_c rows each, then an atom a lane;
-    // warp 10: the two 128-byte halves of the stage's tokens.
-    const bool is_b = warp == kPairBWarp;
+    // A: lanes 0 .. MB-1 a block of 128 a_c rows each, then an atom a lane;
+    // B: the stage's tokens in boxes 128 bytes wide.
+    const bool is_b = warp == kScaledBWarp;
     if (is_b || !P.static_weights) griddep_wait();
     const bool is_a = !is_b && lane < MB;
-    const int el = lane - MB;                           // block el / 2, atom el % 2
-    const int lanes = is_b ? 2 : 3 * MB;
+    const int el = lane - MB;                           // block el / ATOMS, its atom el % ATOMS
+    const int lanes = is_b ? C::B_BOXES : MB + MB * C::ATOMS;
     const CUtensorMap* map = is_b ? &tmB : is_a ? &tmA : &tmE;
     const uint32_t off = is_b   ? C::A_BYTES + lane * C::B_BOX
                          : is_a ? lane * C::A_BOX
                                 : C::A_BYTES + C::B_BYTES + el * kAtomBytes;
     const int dx = is_b ? C::BKD : is_a ? C::BKD / 2 : 0;
-    const int dy = is_b || is_a ? 0 : 2 * P.meta_mblocks * 8;
+    const int dy = is_b || is_a ? 0 : C::ATOMS * P.meta_mblocks * 8;
     const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);
     int s = 0;
     uint32_t ph = 0;
@@ -213,8 +259,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         y = (mt * MB + lane) * 256 + prank * 128;
       } else {
         // Blocks past the image belong to rows past m: any valid codes serve.
-        const int mb = min((mt * MB + (el >> 1)) * 2 + prank, P.meta_mblocks - 1);
-        y = ((el & 1) * P.meta_mblocks + mb) * 8;
+        const int mb = min((mt * MB + el / C::ATOMS) * 2 + prank, P.meta_mblocks - 1);
+        y = ((el % C::ATOMS) * P.meta_mblocks + mb) * 8;
       }
       for (int ks = 0; ks < P.k_stages; ++ks) {
         int good = 1;
@@ -240,7 +286,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       for (int i = 0; i < C::STAGES; ++i)
         if (used_mask & (1u << i)) mbar_wait(&full_bar[i], (used_ph >> i) & 1u, &dummy, tmo);
     }
-  } else if (warp == 1) {
+  } else if (warp == kScaledMmaWarp) {
     // ------------------------------------------------------------ MMA issuer (leader)
     if (leader) {
       const uint32_t base = smem_u32(smem);
@@ -248,7 +294,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const uint64_t bdesc0 = make_sdesc(base + C::A_BYTES, 16, 1024, kLayoutSW128);
       const uint64_t edesc0 = make_sdesc(base + C::A_BYTES + C::B_BYTES, kAtomBytes, 128, kLayoutNone);
       int s = 0;
-      uint32_t ph = 0, aph = 0, ebuf = 0;
+      uint32_t ph = 0, aph = 0, ebuf = 0, acc0 = 0;   // acc0: this tile's first accumulator
       bool ok = true, any = false;
       for (int t = pair; t < num_tiles && ok; t += npairs) {
         int mt, nt;
@@ -266,25 +312,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           const uint64_t so = static_cast<uint64_t>(s * (C::STAGE_BYTES >> 4));
           if (elect_one()) {
 #pragma unroll
-            for (int a = 0; a < MB * 2; ++a) tc_cp<2>(e + 4 * a, edesc0 + so + a * (kAtomBytes >> 4));
+            for (int a = 0; a < MB * C::ATOMS; ++a) tc_cp<2>(e + 4 * a, edesc0 + so + a * (kAtomBytes >> 4));
           }
           __syncwarp();
 #pragma unroll
           for (int b = 0; b < MB; ++b) {
             if (ks == 0) {   // this accumulator's columns of the last tile are in registers
-              if (!mbar_wait_warp<true>(&acce_bar[b], aph ^ 1u, &abort_sh, tmo)) {
+              if (!mbar_wait_warp<true>(&acce_bar[acc0 + b], aph ^ 1u, &abort_sh, tmo)) {
                 ok = false;
                 break;
               }
               tc_fence_after();
             }
-            if (elect_one()) {
+            if ((mt * MB + b) * 256 < P.m && elect_one()) {
 #pragma unroll
               for (int j = 0; j < C::MMAS; ++j)
                 if (j * 64 < kleft) {   // past K there is no metadata
                   const uint64_t ad = adesc0 + so + b * (C::A_BOX >> 4) + j * 2;
                   const uint64_t bd = bdesc0 + so + (j >> 1) * (C::B_BOX >> 4) + (j & 1) * 4;
-                  const uint32_t d = tmem_base + b * 256, ec = e + b * 8 + j * 2;
+                  const uint32_t d = tmem_base + (acc0 + b) * 256, ec = e + b * C::ATOMS * 4 + j * 2;
                   const uint32_t acc = (ks > 0 || j > 0) ? 1u : 0u;
                   if constexpr (I8) tc_mma_sp_pair_i8(d, ad, bd, ec, C::IDESC, acc);
                   else tc_mma_sp_pair<1>(d, ad, bd, ec, C::IDESC, acc);
@@ -299,9 +345,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           if (++s == C::STAGES) s = 0, ph ^= 1u;
         }
         if (!ok) break;
-        if (elect_one()) tc_commit_pair(&accf_bar, 3);
+        if (elect_one()) tc_commit_pair(&accf_bar[MB == 1 ? acc0 : 0], 3);
         __syncwarp();
-        aph ^= 1u;
+        if (MB == 1) acc0 ^= 1u;
+        if (acc0 == 0) aph ^= 1u;
       }
       if (!ok && any) {
         volatile int dummy = 0;
@@ -311,17 +358,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         __syncwarp();
       }
     }
-  } else {
+  } else if (warp < kPairEpiWarps) {
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;
-    const int half = (warp - 2) >> 2;
+    const int half = warp >> 2;
     const uint32_t acce0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
-    uint32_t aph = 0;
+    uint32_t aph = 0, acc0 = 0;
     griddep_wait();   // scales and bias may come from the previous kernel
     for (int t = pair; t < num_tiles; t += npairs) {
       int mt, nt;
       scaled_tile(P, t, mt, nt);
-      float* sn = sn_sh[warp - 2];
+      float* sn = sn_sh[warp];
       __syncwarp();
       for (int j = lane; j < C::CW; j += 32) {
         const int tok = nt * BN + half * C::CW + j;
@@ -329,36 +376,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
       __syncwarp();
       bool ok = true;
-      if (lane == 0) ok = mbar_wait_sleepy(&accf_bar, aph, &abort_sh, tmo);
+      if (lane == 0) ok = mbar_wait_sleepy(&accf_bar[MB == 1 ? acc0 : 0], aph, &abort_sh, tmo);
       if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) == 0) break;
       tc_fence_after();
-      aph ^= 1u;
       const int t0 = nt * BN + half * C::CW;
 #pragma unroll 1
       for (int b = 0; b < MB; ++b) {
         uint32_t r[C::CW];
         const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
-                            static_cast<uint32_t>(b * 256 + half * C::CW);
+                            (acc0 + b) * 256 + half * C::CW;
 #pragma unroll
-        for (int c = 0; c < C::CW; c += 16)
-          tmem_ld_x16(tb + c, *reinterpret_cast<uint32_t(*)[16]>(&r[c]));
+        for (int c = 0; c < C::CW; c += 16) tmem_ld_x16(tb + c, *reinterpret_cast<uint32_t(*)[16]>(&r[c]));
         tmem_ld_wait(r);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(acce0 + b * sizeof(uint64_t));
+        if (lane == 0) mbar_arrive_cluster(acce0 + (acc0 + b) * sizeof(uint64_t));
         const int row = (mt * MB + b) * 256 + prank * 128 + q * 32 + lane;
-        const bool paired = P.words && t0 + C::CW <= P.n && row - lane + 32 <= P.m;
-        if (P.out_type == 2) scaled_emit<I8, C::CW, 2>(P, r, row, t0, sn, paired);
-        else if (P.out_type == 1) scaled_emit<I8, C::CW, 1>(P, r, row, t0, sn, paired);
-        else scaled_emit<I8, C::CW, 0>(P, r, row, t0, sn, paired);
+        if (row - lane >= P.m) continue;
+        if (P.out_type == 2) scaled_emit<I8, C::CW, 2>(P, r, row, t0, sn);
+        else if (P.out_type == 1) scaled_emit<I8, C::CW, 1>(P, r, row, t0, sn);
+        else scaled_emit<I8, C::CW, 0>(P, r, row, t0, sn);
       }
+      if (MB == 1) acc0 ^= 1u;
+      if (acc0 == 0) aph ^= 1u;
     }
   }
 
   tc_fence_before();
   __syncthreads();
   cluster_sync();
-  if (warp == 1) {
+  if (warp == kScaledMmaWarp) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);
   }

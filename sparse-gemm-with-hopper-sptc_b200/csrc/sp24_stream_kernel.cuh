@@ -36,6 +36,7 @@ struct StreamParams {
   int m_blocks;
   int splits;               // S
   int stages;               // K stages over all splits
+  int ring;                 // slots, at most C::STAGES
   const uint8_t* meta;      // scaled: tcgen05 metadata image
   int meta_mblocks, katoms;
   const float *scale_m, *scale_n, *bias;
@@ -71,6 +72,7 @@ struct StreamCfg {
   static constexpr int STAGES_RAW = (kSmemBudget - 1024) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
+  static constexpr int PARKED = G * BN * (kBlockM + 4) * 4;   // a partial tile, in the idle ring
   static constexpr int LOADS = G + B_BOXES + ATOMS;
   static constexpr int E_COL = G * BN;
   static constexpr int COLS_NEEDED = E_COL + 2 * ATOMS * 4;
@@ -89,7 +91,7 @@ struct StreamCfg {
   static constexpr int RS = kBlockM + 4;                 // parked column stride (words)
   static_assert(BN % 16 == 0 && BN >= 16 && BN <= 128, "token tile");
   static_assert(STAGE_BYTES % 1024 == 0, "stage regions must stay 1024-aligned");
-  static_assert(G * BN * RS * 4 <= STAGES * STAGE_BYTES, "parked partial tiles must fit the ring");
+  static_assert(PARKED <= STAGES * STAGE_BYTES, "parked partial tiles must fit the ring");
 };
 
 template <int OP>
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 
   if (threadIdx.x == 0) {
     abort_sh = 0;
-    for (int s = 0; s < C::STAGES; ++s) {
+    for (int s = 0; s < P.ring; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     mbar_init(&drain_bar, 1);
     fence_barrier_init();
     // Armed here for the first use, by the MMA warp for later ones.
-    for (int s = 0; s < C::STAGES && s < nst; ++s) mbar_arrive_expect_tx(&full_bar[s], stage_tx(g0 + s));
+    for (int s = 0; s < P.ring && s < nst; ++s) mbar_arrive_expect_tx(&full_bar[s], stage_tx(g0 + s));
   }
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmA);
@@ -223,15 +225,15 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                     &full_bar[slot]);
       }
     };
-    const int pre = min(C::STAGES, nst);
+    const int pre = min(P.ring, nst);
     const bool loads = lane < C::LOADS;
     if (P.static_weights && loads && !is_b)
       for (int i = 0; i < pre; ++i) issue(i, g0 + i);
     griddep_wait();
     if (loads && (is_b || !P.static_weights))
       for (int i = 0; i < pre; ++i) issue(i, g0 + i);
-    int s = pre % C::STAGES;
-    uint32_t ph = pre == C::STAGES ? 1u : 0u;
+    int s = pre == P.ring ? 0 : pre;
+    uint32_t ph = pre == P.ring ? 1u : 0u;
     uint32_t used_mask = (1u << pre) - 1u, used_ph = 0;
     bool ok = true;
     for (int i = pre; i < nst; ++i) {
@@ -243,12 +245,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       }
       if (loads) issue(s, g0 + i);
       used_ph = (used_ph & ~(1u << s)) | (ph << s);
-      if (++s == C::STAGES) s = 0, ph ^= 1u;
+      if (++s == P.ring) s = 0, ph ^= 1u;
     }
     if (!ok && lane == 0) {
       // Error path: copies in flight land before the CTA leaves.
       volatile int dummy = 0;
-      for (int j = 0; j < C::STAGES; ++j)
+      for (int j = 0; j < P.ring; ++j)
         if (used_mask & (1u << j)) mbar_wait(&full_bar[j], (used_ph >> j) & 1u, &dummy, tmo);
     }
   } else if (warp == 1) {
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         ok = false;
         break;
       }
-      if (lane == 0 && i + C::STAGES < nst) mbar_arrive_expect_tx(&full_bar[s], stage_tx(g + C::STAGES));
+      if (lane == 0 && i + P.ring < nst) mbar_arrive_expect_tx(&full_bar[s], stage_tx(g + P.ring));
       tc_fence_after();
       ebuf ^= static_cast<uint32_t>(C::ATOMS * 4);
       const uint32_t e = tmem_base + static_cast<uint32_t>(C::E_COL) + ebuf;
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       }
       __syncwarp();
       any = true;
-      if (++s == C::STAGES) s = 0, ph ^= 1u;
+      if (++s == P.ring) s = 0, ph ^= 1u;
     }
     if (ok && elect_one()) tc_commit(&accf_bar);
     __syncwarp();

@@ -227,7 +227,8 @@ def check_scaled(c, x, w, sw, sx, bias, qdtype, k):
     (31, 640, 512), (32, 384, 2048), (33, 255, 256), (64, 1024, 1024), (65, 130, 704),
     (100, 2000, 128), (127, 256, 256), (128, 128, 1024), (129, 512, 192), (200, 300, 4096),
     (255, 257, 512), (256, 256, 256), (257, 511, 320), (300, 2304, 1088), (513, 769, 640),
-    (1000, 1000, 1024), (64, 4096, 14336), (3, 14336, 4096)])
+    (1000, 1000, 1024), (64, 4096, 14336), (3, 14336, 4096),
+    (33, 14336, 320), (128, 14080, 192), (1000, 14336, 192), (1111, 14081, 320), (2049, 9000, 64)])
 def test_scaled_sizes(n, m, k, qdtype):
     a_c, image, w = weights_2of4(m, k, qdtype, seed=m + k)
     x = tokens_8bit(n, k, qdtype, seed=n)
