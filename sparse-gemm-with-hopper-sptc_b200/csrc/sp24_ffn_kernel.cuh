@@ -41,6 +41,7 @@ struct FfnParams {
   int k_stages;            // 64-deep stages of one tile
   int plane;               // dx: stages per plane; dw: row tiles per plane
   int group_m;
+  int splits;              // K-split form: pairs per cluster
   void *out0, *out1;       // dw: dw_gate, dw_up; else out0
   long long ld_out0, ld_out1;
   int vec_out;             // 2: rows start on 32 bytes, 1: on 16, 0: neither
@@ -89,56 +90,62 @@ struct FfnCfg {
   static constexpr uint32_t A_STEP = A_MN ? 16 * 128 : 32;
   static constexpr uint32_t B_STEP = B_MN ? 16 * 128 : 32;
   static constexpr uint32_t IDESC = make_idesc_dense(DT == 1 ? 1 : 0, 256, 256, A_MN, B_MN);
-  static constexpr int TILE_N = MODE == kFfnForward ? 128 : 256;   // output columns of a tile
+  static constexpr int RS = 256 + 4;                  // parked partial row stride (floats)
+  static_assert(128 * RS * 4 <= STAGES * STAGE_BYTES, "a parked partial tile fits the ring");
 };
 
 // Warp-collective: 64 consecutive 16-bit columns of the lane's own row, as 32
-// words of two; the warp's rows are row0 .. row0 + 31 and rows >= m are absent.
-// Full runs on 16-byte rows leave as 128-byte pieces through the quad
-// transpose (sp24_gemm2sm_kernel.cuh); the rest goes element by element.
+// words of two; the warp's rows are row0 .. row0 + 31 and rows >= m and columns
+// >= n are absent.  After the quad transpose (sp24_gemm2sm_kernel.cuh) four lanes
+// hold one row's 128 bytes between them and store them in one piece; a ragged
+// end costs the last eight columns' lane single elements.
 SP24_DEV void store_run64(void* out, long long ld, int vec, uint32_t (&u)[32], int row0, int m,
                           int col0, int n) {
+  if (col0 >= n) return;   // warp-uniform
   const int lane = threadIdx.x & 31;
-  if (vec > 0 && col0 + 64 <= n) {
-    quad_transpose_units(u);
-    const int p = lane & 3, g = lane >> 2;
+  quad_transpose_units(u);
+  const int c = col0 + 16 * (lane & 3), g = lane >> 2;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int row = row0 + 4 * g + q;
-      if (row < m) {
-        uint16_t* dst = static_cast<uint16_t*>(out) + row * ld + col0 + 16 * p;
-        if (vec == 2) {
-          st_global_v8_u32(dst, &u[8 * q]);
-        } else {
-          *reinterpret_cast<uint4*>(dst) = make_uint4(u[8 * q], u[8 * q + 1], u[8 * q + 2], u[8 * q + 3]);
-          *reinterpret_cast<uint4*>(dst + 8) =
-              make_uint4(u[8 * q + 4], u[8 * q + 5], u[8 * q + 6], u[8 * q + 7]);
-        }
+  for (int q = 0; q < 4; ++q) {
+    const int row = row0 + 4 * g + q;
+    if (row >= m) continue;
+    uint16_t* dst = static_cast<uint16_t*>(out) + row * ld + c;
+    if (vec == 2 && c + 16 <= n) {
+      st_global_v8_u32(dst, &u[8 * q]);
+      continue;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t* w = &u[8 * q + 4 * h];
+      if (vec > 0 && c + 8 * h + 8 <= n) {
+        *reinterpret_cast<uint4*>(dst + 8 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + 8 * h + j < n) dst[8 * h + j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
       }
     }
-  } else if (row0 + lane < m) {
-    uint16_t* dst = static_cast<uint16_t*>(out) + (row0 + lane) * ld + col0;
-#pragma unroll
-    for (int j = 0; j < 64; ++j)
-      if (col0 + j < n) dst[j] = static_cast<uint16_t>(u[j / 2] >> (16 * (j & 1)));
   }
 }
 
-// The same for 32 fp32 columns on rows that start on 32 bytes.
+// The same for 32 fp32 columns on rows that start on 32 bytes and are padded to
+// multiples of eight: whole units of eight, the last one over the padding.
 SP24_DEV void store_run32_f32(float* out, long long ld, uint32_t (&u)[32], int row0, int m, int col0,
                               int n) {
+  if (col0 >= n) return;
   const int lane = threadIdx.x & 31;
-  if (col0 + 32 <= n) {
-    store_rows_128b(out + col0, ld * 4, u, row0, m, false, 0);
-  } else if (row0 + lane < m) {
-    float* dst = out + (row0 + lane) * ld + col0;
+  quad_transpose_units(u);
+  const int c = col0 + 8 * (lane & 3), g = lane >> 2;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col0 + j < n) dst[j] = __uint_as_float(u[j]);
+  for (int q = 0; q < 4; ++q) {
+    const int row = row0 + 4 * g + q;
+    if (row < m && c < n) st_global_v8_u32(out + row * ld + c, &u[8 * q]);
   }
 }
 
-SP24_DEV float gate_act(float g, int silu_on) { return silu_on ? silu(g) : g; }
+// The approximate quotient: the IEEE division takes its slow path for the zeroes
+// of absent rows (one 256 x 128 tile, 255 of its rows present: 16.9 -> 5.1 us).
+SP24_DEV float gate_act(float g, int silu_on) { return silu_on ? silu_of(g) : g; }
 
 SP24_DEV void ffn_tile(const FfnParams& P, int t, int& mt, int& nt) {
   const int per_group = P.group_m * P.n_tiles;
@@ -153,11 +160,13 @@ SP24_DEV void ffn_tile(const FfnParams& P, int t, int& mt, int& nt) {
 // tmA0 / tmA1, tmB0 / tmB1: the operands' two planes (forward: A is x, B0 and B1
 // are Wg and Wu; dx: A planes dg and du, B planes Wg and Wu; dw: A planes dg
 // and du, B is x).
-template <int DT, int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-    ffn_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
-                    const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
-                    const FfnParams P) {
+// KS = 0: clusters of 2, persistent over the tiles.  KS = 1 (few tiles): a
+// cluster of 2 S CTAs computes one tile, pair p its K slice p; each CTA parks its
+// fp32 partial tile in its idle ring, and the pairs' partials are summed in
+// order over distributed shared memory.
+template <int DT, int MODE, int KS>
+SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, const CUtensorMap& tmB0,
+                            const CUtensorMap& tmB1, const FfnParams& P) {
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
   using C = FfnCfg<DT, MODE>;
   extern __shared__ uint8_t smem_raw[];
@@ -173,11 +182,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                                              ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int prank = static_cast<int>(cluster_ctarank());
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t lead = KS ? (rank & ~1u) : 0u;   // cluster rank of this pair's leader
+  const int prank = static_cast<int>(rank - lead);
   const bool leader = prank == 0;
-  const int pair = static_cast<int>(blockIdx.x >> 1);
-  const int npairs = static_cast<int>(gridDim.x >> 1);
+  const uint16_t pair_mask = static_cast<uint16_t>(3u << lead);
+  const int pair = KS ? static_cast<int>(blockIdx.x) / (2 * P.splits) : static_cast<int>(blockIdx.x >> 1);
   const int num_tiles = P.m_tiles * P.n_tiles;
+  const int npairs = KS ? num_tiles : static_cast<int>(gridDim.x >> 1);   // KS: one tile
+  const int split = KS ? static_cast<int>(rank >> 1) : 0;
+  const int ks0 = KS ? P.k_stages * split / P.splits : 0;
+  const int ks1 = KS ? P.k_stages * (split + 1) / P.splits : P.k_stages;
   const uint64_t tmo = P.timeout_ns;
 
   if (threadIdx.x == 0) {
@@ -220,7 +235,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const bool is_b = warp == kPairBWarp;
     const bool mn = is_b ? C::B_MN : C::A_MN;
     const int boxes = is_b ? C::B_BOXES : C::A_BOXES;
-    const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);
+    const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), lead);
     const uint32_t off = (is_b ? C::OPERAND : 0) + lane * (C::OPERAND / 2);
     int s = 0;
     uint32_t ph = 0;
@@ -234,7 +249,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       // First row (or, MN-major, first column) of this CTA's 128.
       const int first = is_b ? (MODE == kFfnForward ? nt * 128 : nt * 256 + prank * 128)
                              : mt * 256 + prank * 128;
-      for (int ks = 0; ks < P.k_stages; ++ks) {
+      for (int ks = ks0; ks < ks1; ++ks) {
         int good = 1;
         if (lane == 0) good = mbar_wait_fast(&empty_bar[s], ph ^ 1u, &abort_sh, tmo) ? 1 : 0;
         if (__shfl_sync(0xffffffffu, good, 0) == 0) {
@@ -279,7 +294,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
         tc_fence_after();
         const uint32_t d = tmem_base + static_cast<uint32_t>(buf * 256);
-        for (int ks = 0; ks < P.k_stages; ++ks) {
+        for (int ks = ks0; ks < ks1; ++ks) {
           if (!mbar_wait_warp(&full_bar[s], ph, &abort_sh, tmo)) {
             ok = false;
             break;
@@ -292,22 +307,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             for (int j = 0; j < C::BK / 16; ++j)
               tc_mma_dense_pair(d, adesc0 + so + j * (C::A_STEP >> 4),
                                 bdesc0 + so + j * (C::B_STEP >> 4), C::IDESC,
-                                (ks > 0 || j > 0) ? 1u : 0u);
-            tc_commit_pair(&empty_bar[s], 3);
+                                (ks > ks0 || j > 0) ? 1u : 0u);
+            tc_commit_pair(&empty_bar[s], pair_mask);
           }
           __syncwarp();
           any = true;
           if (++s == C::STAGES) s = 0, ph ^= 1u;
         }
         if (!ok) break;
-        if (elect_one()) tc_commit_pair(&accf_bar[buf], 3);
+        if (elect_one()) tc_commit_pair(&accf_bar[buf], pair_mask);
         __syncwarp();
         buf ^= 1;
         if (buf == 0) aph ^= 1u;
       }
       if (!ok && any) {
         volatile int dummy = 0;
-        if (elect_one()) tc_commit_pair(&drain_bar, 1);
+        if (elect_one()) tc_commit_pair(&drain_bar, static_cast<uint16_t>(1u << lead));
         __syncwarp();
         if (lane == 0) mbar_wait(&drain_bar, 0, &dummy, tmo);
         __syncwarp();
@@ -317,7 +332,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;             // TMEM lane quarter
     const int half = (warp - 2) >> 2;   // which half of the tile's columns
-    uint32_t acce0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
+    const uint32_t acce0 = mapa_shared(smem_u32(&acce_bar[0]), lead);
     int buf = 0;
     uint32_t aph = 0;
     for (int t = pair; t < num_tiles; t += npairs) {
@@ -347,7 +362,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(acce0 + buf * sizeof(uint64_t));
         }
-        if constexpr (MODE == kFfnForward) {
+        if constexpr (KS) {
+          float* red = reinterpret_cast<float*>(smem) + (q * 32 + lane) * C::RS + half * 128 + c * 64;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            *reinterpret_cast<uint4*>(red + j) = make_uint4(r0[j], r0[j + 1], r0[j + 2], r0[j + 3]);
+            *reinterpret_cast<uint4*>(red + 32 + j) = make_uint4(r1[j], r1[j + 1], r1[j + 2], r1[j + 3]);
+          }
+        } else if constexpr (MODE == kFfnForward) {
           const int col0 = nt * 128 + half * 64;
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
@@ -379,13 +401,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  cluster_sync();
+  cluster_sync();   // KS: every pair's partial is parked and visible (release / acquire)
+  if constexpr (KS) {
+    // CTA (slice p, half h) finishes rows [128 p / S, 128 (p + 1) / S) of its half
+    // of the tile, four columns a thread.
+    static_assert(MODE == kFfnDx, "the K-split form serves dx");
+    const int S = P.splits;
+    int mt, nt;
+    ffn_tile(P, pair, mt, nt);
+    const int r0 = 128 * split / S, rows = 128 * (split + 1) / S - r0;
+    const float* red = reinterpret_cast<const float*>(smem);
+    for (int i = threadIdx.x; i < rows * 64; i += kPairThreads) {
+      const int rl = r0 + (i >> 6), cl = (i & 63) * 4;
+      const uint32_t la = smem_u32(red + rl * C::RS + cl);
+      float4 a = ld_dsmem_f4(mapa_shared(la, static_cast<uint32_t>(prank)));
+      for (int sp = 1; sp < S; ++sp) {
+        const float4 v = ld_dsmem_f4(mapa_shared(la, static_cast<uint32_t>(2 * sp + prank)));
+        a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+      }
+      const int row = mt * 256 + prank * 128 + rl, col = nt * 256 + cl;
+      if (row >= P.m) continue;
+      uint16_t* dst = static_cast<uint16_t*>(P.out0) + row * P.ld_out0 + col;
+      const uint32_t w[2] = {pack16<DT>(a.x, a.y), pack16<DT>(a.z, a.w)};
+      if (P.vec_out > 0 && col + 4 <= P.n) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < P.n) dst[j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+      }
+    }
+    cluster_sync();   // no CTA leaves while others still read its shared memory
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);
   }
   if (threadIdx.x == 0 && abort_sh != 0 && P.status != nullptr) atomicExch(P.status, 1);
 #endif
+}
+
+template <int DT, int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    ffn_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
+                    const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
+                    const FfnParams P) {
+  ffn_pair_body<DT, MODE, 0>(tmA0, tmA1, tmB0, tmB1, P);
+}
+
+// Launched with a run-time cluster of 2 * P.splits CTAs.
+template <int DT>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    ffn_dx_split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
+                        const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
+                        const FfnParams P) {
+  ffn_pair_body<DT, kFfnDx, 1>(tmA0, tmA1, tmB0, tmB1, P);
 }
 
 // dg = d_out u act'(g) and du = d_out act(g) from the saved fp32 sums, rounded

@@ -206,6 +206,40 @@ sp24_status launch_ffn_pair(const FfnCall& c, const CUtensorMap (&a)[2], const C
                             a[0], a[1], b[0], b[1], p);
 }
 
+// The largest number of K splits, at most `want`, whose clusters (`per_split`
+// CTAs each) are all resident at once: a second wave of clusters would cost
+// more than the split saves.
+template <typename Kern>
+int resident_splits(Kern kern, int threads, int smem, long long clusters, int per_split, int want) {
+  static std::atomic<int> cache[kMaxDevices][9];   // by CTAs per cluster; 0 = not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 1;
+  for (int s = want; s > 1; --s) {
+    std::atomic<int>& slot = cache[dev][s * per_split];
+    int n = slot.load(std::memory_order_relaxed);
+    if (n == 0) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(static_cast<unsigned>(s * per_split));
+      cfg.blockDim = dim3(static_cast<unsigned>(threads));
+      cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = static_cast<unsigned>(s * per_split);
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();
+        n = 0;
+      }
+      n = n > 0 ? n : -1;
+      slot.store(n, std::memory_order_relaxed);
+    }
+    if (n >= clusters) return s;
+  }
+  return 1;
+}
+
 // Tensor map of a 16-bit matrix in boxes of 64 columns (128 bytes).
 sp24_status encode_16(CUtensorMap* map, const void* base, int rows, int cols, int64_t ld, int box_rows) {
   return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, static_cast<uint64_t>(cols),
@@ -228,8 +262,8 @@ sp24_status launch_stream_bn(const FfnCall& c, const CUtensorMap& a, const CUten
   const int n_tiles = (p.n + BN - 1) / BN;
   const long long tiles = static_cast<long long>(p.m_blocks) * n_tiles;
   if (tiles * sp24::kStreamMaxSplits > 0x7fffffff) return SP24_ERR_SHAPE;
-  p.splits = static_cast<int>(std::max(1LL, std::min<long long>({c.sm_count / tiles, sp24::kStreamMaxSplits,
-                                                                 p.stages})));
+  const int want = static_cast<int>(std::min<long long>({c.sm_count / tiles, sp24::kStreamMaxSplits, p.stages}));
+  p.splits = resident_splits(kern, sp24::kStreamThreads, C::SMEM_BYTES, tiles, 1, want);
   // No more slots than a CTA has stages: what is left of the SM's shared memory
   // lets the next kernel's CTAs start their prologue beside this one's tail
   // (4096 x 4096, 1 token, back to back: 6.1 -> 5.6 us).
@@ -366,11 +400,32 @@ sp24_status ffn_forward(const FfnCall& c, const sp24_ffn_desc* d, void* out, int
   p.m = d->t, p.n = d->f;
   p.m_tiles = (d->t + 255) / 256, p.n_tiles = (d->f + 127) / 128;
   p.k_stages = (d->h + 63) / 64;
-  p.group_m = 8;
+  p.group_m = 16;
   p.out0 = out, p.ld_out0 = ld_out, p.vec_out = out_vec(out, ld_out);
   p.saved = static_cast<float*>(d->saved), p.ld_saved = ffn_ld(d->f);
   p.silu = d->act == SP24_ACT_SILU;
   return launch_ffn_pair<DT, sp24::kFfnForward>(c, a, b, p);
+}
+
+template <int DT>
+sp24_status launch_dx_split(const FfnCall& c, const CUtensorMap (&a)[2], const CUtensorMap (&b)[2],
+                            sp24::FfnParams p) {
+  p.status = c.status;
+  p.timeout_ns = kDefaultTimeoutNs;
+  return launch_gemm_kernel(sp24::ffn_dx_split_kernel<DT>,
+                            static_cast<unsigned>(p.m_tiles * p.n_tiles * 2 * p.splits), sp24::kPairThreads,
+                            sp24::FfnCfg<DT, sp24::kFfnDx>::SMEM_BYTES, c.stream,
+                            static_cast<unsigned>(2 * p.splits), true, a[0], a[1], b[0], b[1], p);
+}
+
+// Pairs per cluster of the K-split dx; 1 where the form does not apply.
+template <int DT>
+int dx_splits(long long tiles, int want) {
+  constexpr int smem = sp24::FfnCfg<DT, sp24::kFfnDx>::SMEM_BYTES;
+  static std::atomic<bool> attr_set[kMaxDevices];
+  auto kern = sp24::ffn_dx_split_kernel<DT>;
+  if (ensure_kernel_attrs(kern, attr_set, smem) != SP24_OK) return 1;
+  return resident_splits(kern, sp24::kPairThreads, smem, tiles, 2, want);
 }
 
 template <int DT>
@@ -400,7 +455,12 @@ sp24_status ffn_backward(const FfnCall& c, const sp24_ffn_desc* d, const sp24_ff
     p.plane = (d->f + 63) / 64, p.k_stages = 2 * p.plane;
     p.group_m = 8;
     p.out0 = g->dx, p.ld_out0 = stride_or(g->ld_dx, d->h), p.vec_out = out_vec(g->dx, p.ld_out0);
-    st = launch_ffn_pair<DT, sp24::kFfnDx>(c, a, b, p);
+    // Few tiles: K split over the pairs of a cluster (777 x 1000, f = 2744, 16
+    // tiles of 86 stages: 48 -> 19 us with four).
+    const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+    const int want = static_cast<int>(std::min<long long>({c.sm_count / 2 / tiles, 4, p.k_stages}));
+    p.splits = want > 1 ? dx_splits<DT>(tiles, want) : 1;
+    st = p.splits > 1 ? launch_dx_split<DT>(c, a, b, p) : launch_ffn_pair<DT, sp24::kFfnDx>(c, a, b, p);
     if (st != SP24_OK) return st;
   }
   if (g->dw_gate != nullptr) {

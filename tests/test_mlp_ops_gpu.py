@@ -372,7 +372,8 @@ def check_ffn(x, wg, wu, dh, act, out, grads=None):
 @pytest.mark.parametrize("t,h,f", [(1, 8, 8), (1, 64, 128), (1, 1000, 264), (2, 72, 1000), (5, 136, 96), (8, 256, 512),
                                    (16, 4096, 640), (17, 200, 200), (31, 512, 72), (33, 64, 2744), (64, 1024, 256),
                                    (65, 128, 128), (100, 264, 1032), (128, 256, 256), (129, 512, 136), (257, 320, 512),
-                                   (300, 1000, 776), (513, 256, 1024)])
+                                   (300, 1000, 776), (513, 256, 1024),
+                                   (1300, 1280, 264), (1030, 1000, 136), (2600, 264, 512)])
 def test_ffn_sizes(t, h, f, dtype, act):
     x, wg, wu, dh = ffn_inputs(t, h, f, dtype, seed=t + h)
     out, saved = sp24.ffn_gated(x, wg, wu, act=act, save=True)
