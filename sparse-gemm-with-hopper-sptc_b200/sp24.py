@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import (POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_longlong,
                     c_size_t, c_uint8, c_ulonglong, c_void_p)
 
@@ -191,11 +192,11 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.sp24_unshard_columns_f32.argtypes = [c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                              c_void_p]
     for name in ("sp24_rmsnorm_quant", "sp24_swiglu_quant", "sp24_quantize_rows"):
-        getattr(lib, name).argtypes = [POINTER(RowQuantDesc), c_void_p]
+        getattr(lib, name).argtypes = [c_void_p, c_void_p]   # descriptors: byref(...) or packed bytes
         getattr(lib, name).restype = c_int
-    lib.sp24_gemm_scaled.argtypes = [POINTER(ScaledDesc), c_void_p]
-    lib.sp24_ffn_forward.argtypes = [POINTER(FfnDesc), c_void_p, c_int64, c_void_p]
-    lib.sp24_ffn_backward.argtypes = [POINTER(FfnDesc), POINTER(FfnGrads), c_void_p]
+    lib.sp24_gemm_scaled.argtypes = [c_void_p, c_void_p]
+    lib.sp24_ffn_forward.argtypes = [c_void_p, c_void_p, c_int64, c_void_p]
+    lib.sp24_ffn_backward.argtypes = [c_void_p, c_void_p, c_void_p]
     for name in ("sp24_ffn_saved_bytes", "sp24_ffn_workspace_bytes"):
         getattr(lib, name).argtypes = [c_int, c_int]
         getattr(lib, name).restype = c_size_t
@@ -379,7 +380,12 @@ def gemm_fused(a_c, meta, b, m, n, k, *, bias=None, act=ACT_NONE, a_c_up=None, m
 # ------------------------------------------------------------------ the MLP block
 # Activations are token-major: one row per token, its features contiguous.
 # These calls serve single tokens, where the host's time is what counts: shapes
-# and strides are read once, and descriptors are built in one go.
+# and strides are read once, and descriptors are packed in one go (fields and
+# padding as in the structures above).
+_PACK_ROWS = struct.Struct("@4iQqQqQqQqQfQqQ").pack
+_PACK_SCALED = struct.Struct("@5iQqQQqQQQQqQ").pack
+_PACK_FFN = struct.Struct("@5iQqQqQqQNQ").pack
+_PACK_GRADS = struct.Struct("@QqQqQqQqQN").pack
 
 def _rows2d(t, what, cols=None, rows=None):
     """(t, row stride) of a matrix whose rows are contiguous, any row stride;
@@ -474,9 +480,9 @@ def _rows_quant(s, entry, x, qdtype, up, weight, residual, eps):
         p_res, p_total = residual.data_ptr(), total.data_ptr()
     q = torch.empty_like(x, dtype=q_torch) if plain else x.new_empty((rows, cols), dtype=q_torch)
     scale = x.new_empty((rows,), dtype=torch.float32)
-    d = RowQuantDesc(dt, qdtype, rows, cols, x.data_ptr(), ldx, p_up, ld_up, p_res, ld_res,
-                     p_total, 0, p_weight, eps, q.data_ptr(), 0, scale.data_ptr())
-    _check(getattr(_lib or load(), entry)(ctypes.byref(d), s), entry)
+    d = _PACK_ROWS(dt, qdtype, rows, cols, x.data_ptr(), ldx, p_up, ld_up, p_res, ld_res,
+                   p_total, 0, p_weight, eps, q.data_ptr(), 0, scale.data_ptr())
+    _check(getattr(_lib or load(), entry)(d, s), entry)
     return (q, scale) if total is None else (q, scale, total)
 
 
@@ -526,15 +532,16 @@ def _gemm_scaled(s, a_c, meta_tc, x, scale_w, scale_x, bias, out_dtype):
     m, k = a_c.shape[0], 2 * a_c.shape[1]
     x, ldx = _tma_rows(x, "x", k)
     n = x.shape[0]
-    if meta_tc.nbytes != lib.sp24_meta_tc_bytes(m, k):
-        raise ValueError(f"meta_tc: {meta_tc.nbytes} bytes, {meta_tc_bytes(m, k)} expected")
+    image = (m + 255) // 256 * ((k + 127) // 128) * 4096      # sp24_meta_tc_bytes
+    if meta_tc.nbytes != image:
+        raise ValueError(f"meta_tc: {meta_tc.nbytes} bytes, {image} expected")
     scale_w, p_w = _vector_f32(scale_w, m, "scale_w")
     scale_x, p_x = _vector_f32(scale_x, n, "scale_x")
     bias, p_b = _vector_f32(bias, m, "bias")
     c = x.new_empty((n, m), dtype=out_dtype or torch.bfloat16)
-    d = ScaledDesc(code, out, m, n, k, a_c.data_ptr(), lda, meta_tc.data_ptr(), x.data_ptr(), ldx,
-                   p_w, p_x, p_b, c.data_ptr(), 0, 0)
-    _check(lib.sp24_gemm_scaled(ctypes.byref(d), s), "sp24_gemm_scaled")
+    d = _PACK_SCALED(code, out, m, n, k, a_c.data_ptr(), lda, meta_tc.data_ptr(), x.data_ptr(), ldx,
+                     p_w, p_x, p_b, c.data_ptr(), 0, 0)
+    _check(lib.sp24_gemm_scaled(d, s), "sp24_gemm_scaled")
     return c
 
 
@@ -548,8 +555,8 @@ def gemm_scaled(a_c, meta_tc, x, scale_w=None, scale_x=None, *, bias=None, out_d
                meta_tc, x, scale_w, scale_x, bias, out_dtype)
 
 
-def _ffn_desc(x, w_gate, w_up, act, saved=None):
-    """(descriptor, tensors it points to)."""
+def _ffn_args(x, w_gate, w_up, act):
+    """The leading fields of a descriptor, and the tensors they point to."""
     dt = (_codes or _code_tables())["16"].get(x.dtype)
     if dt is None or w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
         raise ValueError(f"ffn_gated: {x.dtype}, {w_gate.dtype}, {w_up.dtype}; one of float16 and "
@@ -559,21 +566,23 @@ def _ffn_desc(x, w_gate, w_up, act, saved=None):
     w_gate, ldg = _tma_rows(w_gate, "w_gate", h)
     f = w_gate.shape[0]
     w_up, ldu = _tma_rows(w_up, "w_up", h, f)
-    p_saved, n_saved = (0, 0) if saved is None else (saved.data_ptr(), saved.nbytes)
-    d = FfnDesc(dt, t, h, f, act, x.data_ptr(), ldx, w_gate.data_ptr(), ldg, w_up.data_ptr(), ldu,
-                p_saved, n_saved, 0)
-    return d, (x, w_gate, w_up)
+    return (dt, t, h, f, act, x.data_ptr(), ldx, w_gate.data_ptr(), ldg, w_up.data_ptr(), ldu), \
+        (x, w_gate, w_up)
 
 
 def _ffn_forward(s, x, w_gate, w_up, act, save):
     import torch
     lib = _lib or load()
-    d, keep = _ffn_desc(x, w_gate, w_up, act)
-    out = x.new_empty((d.t, d.f))
+    args, keep = _ffn_args(x, w_gate, w_up, act)
+    t, f = args[1], args[3]
+    out = x.new_empty((t, f))
+    saved, p_saved, n_saved = None, 0, 0
     if save:
-        saved = x.new_empty((lib.sp24_ffn_saved_bytes(d.t, d.f),), dtype=torch.uint8)
-        d.saved, d.saved_bytes = saved.data_ptr(), saved.nbytes
-    _check(lib.sp24_ffn_forward(ctypes.byref(d), out.data_ptr(), 0, s), "sp24_ffn_forward")
+        n_saved = lib.sp24_ffn_saved_bytes(t, f)
+        saved = x.new_empty((n_saved,), dtype=torch.uint8)
+        p_saved = saved.data_ptr()
+    _check(lib.sp24_ffn_forward(_PACK_FFN(*args, p_saved, n_saved, 0), out.data_ptr(), 0, s),
+           "sp24_ffn_forward")
     del keep
     return (out, saved) if save else out
 
@@ -589,16 +598,18 @@ def _ffn_backward(s, d_out, x, w_gate, w_up, saved, act, need_dx, need_dw):
     lib = _lib or load()
     if d_out.dtype != x.dtype:
         raise ValueError(f"ffn_gated_backward: {d_out.dtype} beside {x.dtype}")
-    d, keep = _ffn_desc(x, w_gate, w_up, act, saved)
-    d_out, ldd = _rows2d(d_out, "d_out", d.f, d.t)
-    dx = x.new_empty((d.t, d.h)) if need_dx else None
+    args, keep = _ffn_args(x, w_gate, w_up, act)
+    _, t, h, f = args[:4]
+    d_out, ldd = _rows2d(d_out, "d_out", f, t)
+    dx = x.new_empty((t, h)) if need_dx else None
     dw_gate = dw_up = None
     if need_dw:
-        dw_gate, dw_up = x.new_empty((d.f, d.h)), x.new_empty((d.f, d.h))
-    ws = x.new_empty((lib.sp24_ffn_workspace_bytes(d.t, d.f),), dtype=torch.uint8)
-    g = FfnGrads(d_out.data_ptr(), ldd, _ptr(dx), 0, _ptr(dw_gate), 0, _ptr(dw_up), 0,
-                 ws.data_ptr(), ws.nbytes)
-    _check(lib.sp24_ffn_backward(ctypes.byref(d), ctypes.byref(g), s), "sp24_ffn_backward")
+        dw_gate, dw_up = x.new_empty((f, h)), x.new_empty((f, h))
+    ws = x.new_empty((lib.sp24_ffn_workspace_bytes(t, f),), dtype=torch.uint8)
+    d = _PACK_FFN(*args, saved.data_ptr(), saved.nbytes, 0)
+    g = _PACK_GRADS(d_out.data_ptr(), ldd, _ptr(dx), 0, _ptr(dw_gate), 0, _ptr(dw_up), 0,
+                    ws.data_ptr(), ws.nbytes)
+    _check(lib.sp24_ffn_backward(d, g, s), "sp24_ffn_backward")
     del keep
     return dx, dw_gate, dw_up
 

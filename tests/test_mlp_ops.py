@@ -150,3 +150,15 @@ def test_shim_refusals():
         sp24.ffn_gated(x, x.half(), x)
     with pytest.raises(ValueError):
         sp24.ffn_gated_backward(x.half(), x, x, x, x)
+
+
+def test_packed_descriptors_match_the_structures():
+    """The shim's packed descriptors are the ctypes structures byte for byte."""
+    for pack, cls in ((sp24._PACK_ROWS, sp24.RowQuantDesc), (sp24._PACK_SCALED, sp24.ScaledDesc),
+                      (sp24._PACK_FFN, sp24.FfnDesc), (sp24._PACK_GRADS, sp24.FfnGrads)):
+        values = [float(i) + 0.5 if t is ctypes.c_float else i + 1 for i, (_, t) in enumerate(cls._fields_)]
+        want = cls(*values)
+        got = pack(*values)
+        assert len(got) <= ctypes.sizeof(cls)
+        back = cls.from_buffer_copy(got.ljust(ctypes.sizeof(cls), b"\0"))
+        assert [getattr(back, n) for n, _ in cls._fields_] == [getattr(want, n) for n, _ in cls._fields_]

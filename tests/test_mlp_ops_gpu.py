@@ -407,7 +407,9 @@ def test_ffn_strides_padding_and_partial_gradients(t):
     assert none_x is None and torch.equal(dwg, full[1]) and torch.equal(dwu, full[2])
     # outputs with odd strides and starts: only their own elements are written
     lib, stream = sp24.load(), torch.cuda.current_stream().cuda_stream
-    d, keep = sp24._ffn_desc(x, wg, wu, sp24.ACT_SILU)
+    d = sp24.FfnDesc()
+    d.dtype, d.t, d.h, d.f, d.act = sp24.F16, t, h, f, sp24.ACT_SILU
+    d.x, d.w_gate, d.w_up = x.data_ptr(), wg.data_ptr(), wu.data_ptr()
     o = torch.full((t, f + 3), 9.0, device=DEV, dtype=dtype)
     assert lib.sp24_ffn_forward(ctypes.byref(d), o.data_ptr() + 2, f + 3, stream) == 0
     d.saved, d.saved_bytes = saved.data_ptr(), saved.numel()
@@ -424,7 +426,6 @@ def test_ffn_strides_padding_and_partial_gradients(t):
     assert flat[0] == 9 and (flat == 9).sum() >= 3 * t
     for b, want in zip(bufs, full):
         assert torch.equal(b[:, :h], want) and torch.all(b[:, h:] == 9)
-    del keep
 
 
 def test_ffn_no_tokens():
@@ -492,3 +493,52 @@ def test_ffn_streams_and_repeats():
         got = sp24.ffn_gated_backward(dh, x, wg, wu, s, stream=side)
         side.synchronize()
         assert torch.equal(o, out) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------ together
+@pytest.mark.parametrize("qdtype,bound", [(sp24.I8, 0.05), (sp24.E4M3, 0.12)])
+def test_example_trains_and_serves(qdtype, bound):
+    """examples/mlp_block.py.  Served error: four roundings to 8 bits (two of
+    activations, two of weights) in quadrature.  int8 rows of normal values
+    (largest near 4 sigma) are off by 4 / 127 / sqrt(12) = 0.9% each; e4m3 by up to
+    2^-4 / sqrt(3) = 3.6% each, less on average; doubled for the norm's and the
+    gate's amplification."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "mlp_block.py")
+    spec = importlib.util.spec_from_file_location("mlp_block", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, errors = example.run(tokens=200, hidden=512, inter=1408, qdtype=qdtype)
+    assert all(b < a for a, b in zip(losses, losses[1:])), losses
+    assert all(e <= bound for e in errors.values()), errors
+
+
+def test_shim_refuses_wrong_types_and_shapes():
+    bf = lambda *s: torch.zeros(*s, device=DEV, dtype=torch.bfloat16)  # noqa: E731
+    i8 = lambda *s: torch.zeros(*s, device=DEV, dtype=torch.int8)  # noqa: E731
+    image = torch.zeros(sp24.meta_tc_bytes(128, 128), device=DEV, dtype=torch.uint8)
+    for call in (lambda: sp24.quantize_rows(bf(4, 64), qdtype=sp24.E5M2),
+                 lambda: sp24.quantize_rows(bf(4, 64).float()),
+                 lambda: sp24.quantize_rows(bf(64)),
+                 lambda: sp24.swiglu_quant(bf(4, 64), bf(4, 64).half()),
+                 lambda: sp24.swiglu_quant(bf(4, 64), bf(4, 72)),
+                 lambda: sp24.rmsnorm_quant(bf(4, 64), bf(72)),
+                 lambda: sp24.rmsnorm_quant(bf(4, 64), bf(64), bf(5, 64)),
+                 lambda: sp24.gemm_scaled(i8(128, 64), image, bf(4, 128)),
+                 lambda: sp24.gemm_scaled(i8(128, 64), image, i8(4, 64)),
+                 lambda: sp24.gemm_scaled(i8(128, 64), image[:-16], i8(4, 128)),
+                 lambda: sp24.gemm_scaled(i8(128, 64), image, i8(4, 128), torch.ones(127, device=DEV)),
+                 lambda: sp24.gemm_scaled(i8(128, 64), image, i8(4, 128), bf(128)),
+                 lambda: sp24.gemm_scaled(i8(128, 64), image, i8(4, 128), out_dtype=torch.int8),
+                 lambda: sp24.gemm_scaled(i8(128, 64), image, torch.zeros(4, 128, dtype=torch.int8)),
+                 lambda: sp24.ffn_gated(bf(4, 64), bf(96, 64), bf(96, 64).half()),
+                 lambda: sp24.ffn_gated(bf(4, 64), bf(96, 64), bf(88, 64)),
+                 lambda: sp24.ffn_gated(bf(4, 64), bf(96, 72), bf(96, 72)),
+                 lambda: sp24.ffn_gated_backward(bf(4, 88), bf(4, 64), bf(96, 64), bf(96, 64), image)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(sp24.Sp24Error):      # k % 64
+        sp24.gemm_scaled(i8(128, 16), image[:2 * 2048], i8(4, 32))
+    with pytest.raises(sp24.Sp24Error):      # a saved buffer of another call
+        sp24.ffn_gated_backward(bf(4, 96), bf(4, 64), bf(96, 64), bf(96, 64), image[:64])
