@@ -53,6 +53,7 @@ sp24_status check_rows(const sp24_rowquant_desc* d, int mode, sp24::RowsParams* 
   p->residual_out = d->residual_out;
   p->weight = d->weight;
   p->eps = d->eps;
+  p->inv_cols = 1.0f / static_cast<float>(d->cols);
   p->q = static_cast<uint8_t*>(d->q);
   p->scale = d->scale;
   return SP24_OK;
@@ -92,21 +93,23 @@ sp24_status launch_rows_vpt(const sp24::RowsParams& p, const DeviceInfo& di, int
   return launch_rows_kernel<DT, MODE, I8, V, VPT, false>(p, di, threads, s);
 }
 
-// Vectors a thread holds.  A row of up to 32 vectors: one, a warp per row (8192
-// x 256 norm: 6.2 us; 7.5 with two, 10.3 with four).  The norm, with its two
-// barriers a row, wants rows spread over more warps than the others (8192 x
-// 4096: 40.7 us with two, 45.2 with four; plain rows 20.6 and 18.6), and so
-// does a call with few rows, whose loads then go out at once (333 x 5000 norm:
-// 6.4 us with two, 7.9 with four).  Single elements (V = 1) want eight: fewer
-// threads, more loads each (4096 x 1001 swiglu: 12.3 us; 12.9 with four).
+// Vectors a thread holds.  The norm waits for a row's two inputs, sum and weight
+// at once and wants many threads with little each: one vector up to 4096 columns
+// (8192 x 4096: 39.0 us; 40.2 with two, 46.1 with four), two up to 16384 (8192 x
+// 8192: 79.9; 85.0 with one, 82.5 with four).  Rows without it have less to keep
+// and more to gain from few warps a row: four (8192 x 4096 plain: 18.5 us; 20.6
+// with two, 22.7 with one), unless a warp covers the row with one (8192 x 256:
+// 4.4 us; 6.0 with four) or there are few rows, whose loads then go out at once.
+// Single elements (V = 1) want eight: fewer threads, more loads each (4096 x 1001
+// swiglu: 10.3 us; 12.0 with four).
 template <int DT, int MODE, int I8, int V>
 sp24_status launch_rows_v(const sp24::RowsParams& p, const DeviceInfo& di, cudaStream_t s) {
   const int vecs = (p.cols + V - 1) / V;
   if constexpr (V == 8) {
-    if (vecs <= 32) return launch_rows_vpt<DT, MODE, I8, V, 1>(p, di, vecs, s);
+    const bool norm = MODE == sp24::kRowsNorm;
+    if (vecs <= (norm ? 512 : 32)) return launch_rows_vpt<DT, MODE, I8, V, 1>(p, di, vecs, s);
     const bool few = p.rows <= 2 * di.sm_count;
-    if ((MODE == sp24::kRowsNorm || few) && vecs <= 2 * 1024)
-      return launch_rows_vpt<DT, MODE, I8, V, 2>(p, di, vecs, s);
+    if ((norm || few) && vecs <= 2 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 2>(p, di, vecs, s);
     if (vecs <= 4 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 4>(p, di, vecs, s);
   } else {
     if (vecs <= 8 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 8>(p, di, vecs, s);

@@ -1,6 +1,12 @@
 // sp24_rows.cuh — rows of 16-bit activations to 8-bit codes with one scale per
 // row: after a residual addition and a root-mean-square norm, after the SwiGLU
 // product, or as they are.
+//
+// Bound by HBM: each input is read once and each output written once.  B200,
+// measured copy rate 6.5 TB/s: norm with residual 8192 x 4096 bf16 (235 MB) 39.0 us,
+// 6.0 TB/s; SwiGLU 4096 x 14336 (294 MB) 49.3 us, 6.0 TB/s; plain 8192 x 14336 (352 MB)
+// 55.7 us, 6.3 TB/s.  The SwiGLU is nearest to another limit: its exponential and
+// reciprocal keep their unit busy half of the time.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -19,10 +25,29 @@ struct RowsParams {
   const void *x, *up, *residual, *weight;
   void* residual_out;
   long long ldx, ld_up, ld_residual, ld_residual_out, ldq;
-  float eps;
+  float eps, inv_cols;
   uint8_t* q;
   float* scale;
 };
+
+// Two fp32 operations in one instruction.
+SP24_DEV uint64_t bits2(float2 a) { return *reinterpret_cast<uint64_t*>(&a); }
+SP24_DEV float2 from_bits2(uint64_t r) { return *reinterpret_cast<float2*>(&r); }
+SP24_DEV float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return from_bits2(r);
+}
+SP24_DEV float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return from_bits2(r);
+}
+SP24_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return from_bits2(r);
+}
 
 template <int DT>
 SP24_DEV float load16(const void* p, long long i) {
@@ -39,8 +64,8 @@ SP24_DEV void store16(void* p, long long i, float v) {
 // rounding step, so the integers stay within +-127; e4m3 saturates.  Integers
 // are rounded by adding 1.5 * 2^23, which leaves v's nearest integer (halves to
 // even) in the low bits of the sum: an addition where a conversion would take
-// the slow unit that the exponentials need (4096 x 14336 SwiGLU: 64 us with
-// conversions, 54 us in e4m3).
+// the slow unit that the exponentials need (4096 x 14336 SwiGLU, before later
+// steps: 63.7 us with conversions, 55.3 with additions).
 template <int I8>
 SP24_DEV uint32_t codes2(float a, float b) {
   if constexpr (I8) {
@@ -58,15 +83,11 @@ SP24_DEV uint4 load_raw(const void* p, long long i) {
   if constexpr (V == 8) return *reinterpret_cast<const uint4*>(q);
   else return make_uint4(*q, 0, 0, 0);
 }
-template <int DT, int V>
-SP24_DEV void unpack_raw(const uint4& w, float (&v)[V]) {
-  const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const uint32_t h = ws[j / 2] >> (16 * (j & 1));
-    if constexpr (DT == 0) v[j] = __half2float(__ushort_as_half(static_cast<unsigned short>(h)));
-    else v[j] = (j & 1) ? __uint_as_float(ws[j / 2] & 0xFFFF0000u) : __uint_as_float(ws[j / 2] << 16);
-  }
+// The two values of one 32-bit word (V = 1: the one value and a zero).
+template <int DT>
+SP24_DEV float2 unpack2(uint32_t w) {
+  if constexpr (DT == 0) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
 template <int DT>
@@ -91,22 +112,36 @@ SP24_DEV float silu_of(float v) {
   return v * r;
 }
 
-// Reduction over the threads of one row: a warp, or the whole block (one
-// barrier; every warp folds the warps' values itself, in the same order).  0
-// is the identity of both uses.  Successive calls alternate between two `sh`.
-template <bool ONE_WARP, typename F>
-SP24_DEV uint32_t row_reduce(uint32_t v, uint32_t* sh, F f) {
+// What the threads of a row agree on.
+struct RowStats {
+  float sum;      // of squares (the norm)
+  uint32_t top;   // bits of the largest magnitude
+};
+
+// Reduces both over the row's threads: a warp, or the whole block with one
+// barrier (every warp folds the warps' values itself, in the same order).
+// Successive rows alternate between two `sh`: a warp can be at most one barrier
+// ahead of another, so none still reads what the next row overwrites.
+template <bool ONE_WARP, bool SUM>
+SP24_DEV RowStats row_reduce(float sum, uint32_t top, uint2* sh) {
+  top = __reduce_max_sync(0xffffffffu, top);
+  if constexpr (SUM) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
   if constexpr (!ONE_WARP) {
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) sh[threadIdx.x >> 5] = v;
+    if (lane == 0) sh[threadIdx.x >> 5] = make_uint2(__float_as_uint(sum), top);
     __syncthreads();
-    v = lane < warps ? sh[lane] : 0u;
+    const uint2 v = lane < warps ? sh[lane] : make_uint2(0, 0);
+    top = __reduce_max_sync(0xffffffffu, v.y);
+    if constexpr (SUM) {
+      sum = __uint_as_float(v.x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
   }
-  return v;
+  return {sum, top};
 }
 
 // max(a, |b|), NaN if either is: its bits then order above infinity's.
@@ -121,28 +156,34 @@ SP24_DEV void cp_async16(void* dst, const void* src) {
 }
 SP24_DEV void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Scale of a row from the bits of its largest |y| (these order as unsigned
-// numbers, infinity and NaN on top), and the factor that gives its codes.
+// The factor that turns a row's values into codes, from the bits of the largest
+// magnitude (these order as unsigned numbers, infinity and NaN on top), and the
+// row's scale for values that are `gain` times those.  Quotients to two ulp.
 struct RowScale {
   float scale, lift, inv;
   bool bad;
 };
 template <int I8>
-SP24_DEV RowScale row_scale(uint32_t mx) {
+SP24_DEV RowScale row_scale(uint32_t top, float gain) {
   constexpr float Q = I8 ? 127.0f : 448.0f;
   RowScale r;
-  const float amax = __uint_as_float(mx);
-  r.bad = mx >= 0x7F800000u;
-  // Q / amax overflows for the smallest rows: those are scaled up first.
-  r.lift = amax < 1e-30f ? 0x1p100f : 1.0f;
-  r.inv = (r.bad || mx == 0) ? 0.0f : Q / (amax * r.lift);
-  r.scale = r.bad ? __uint_as_float(0x7FC00000u) : amax / Q;
+  const float amax = __uint_as_float(top);
+  // The approximate quotient wants its divisor within 2^+-126: rows outside are
+  // brought in first.
+  r.lift = amax < 1e-30f ? 0x1p100f : amax > 1e30f ? 0x1p-40f : 1.0f;
+  const float bounded = amax * r.lift;
+  r.bad = !(bounded < 3e38f) || !(gain == gain);
+  r.inv = (r.bad || top == 0) ? 0.0f : __fdividef(Q, bounded);
+  r.scale = r.bad ? __uint_as_float(0x7FC00000u) : top == 0 ? 0.0f : amax * gain * (1.0f / Q);
   return r;
 }
 
 // One pass over memory: a row's values stay in registers as fp32 from the load
-// to the codes (VPT vectors of V columns a thread), between the two row-wide
-// reductions (the norm's sum of squares, then the largest magnitude).
+// to the codes (VPT vectors of V columns a thread).  The norm's factor
+// r = 1 / sqrt(mean s^2 + eps) is the same for the whole row, so it cancels in
+// the codes: with a = max |s w|, q = round(s w Q / a) and scale = r a / Q.  The sum
+// of squares and the largest magnitude are therefore reduced together, and a
+// row costs one barrier (8192 x 4096: 39.6 us with one after the other).
 // ONE_WARP: a warp per row, blockDim.x / 32 rows a block; else a block per row.
 //
 // The grid is resident and walks the rows.  With V = 8 every thread has a slot
@@ -153,7 +194,8 @@ SP24_DEV RowScale row_scale(uint32_t mx) {
 template <int DT, int MODE, int I8, int V, int VPT, bool ONE_WARP>
 __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_quant_kernel(const RowsParams P) {
   extern __shared__ uint4 slots[];   // V = 8: [input][VPT][blockDim.x]
-  __shared__ uint32_t sh[2][32];
+  __shared__ uint2 sh[2][32];
+  constexpr int H = V == 8 ? 4 : 1;  // pairs of values a vector
   griddep_launch_dependents();
   const int tid = ONE_WARP ? threadIdx.x & 31 : threadIdx.x;
   const int step = ONE_WARP ? 32 : blockDim.x;
@@ -165,28 +207,32 @@ __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_quant_kernel(const
   const bool two = MODE == kRowsSwiglu || (MODE == kRowsNorm && other != nullptr);
   uint4* mine = slots + threadIdx.x;
   auto fetch = [&](long long row) {
+    const uint16_t* px = static_cast<const uint16_t*>(P.x) + row * P.ldx;
+    const uint16_t* po = static_cast<const uint16_t*>(other) + row * ld_other;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = (tid + i * step) * V;
       if (c < P.cols) {
-        cp_async16(mine + i * blockDim.x, static_cast<const uint16_t*>(P.x) + row * P.ldx + c);
-        if (two)
-          cp_async16(mine + (VPT + i) * blockDim.x, static_cast<const uint16_t*>(other) + row * ld_other + c);
+        cp_async16(mine + i * blockDim.x, px + c);
+        if (two) cp_async16(mine + (VPT + i) * blockDim.x, po + c);
       }
     }
   };
   if (r >= P.rows) return;
   griddep_wait();
   if constexpr (V == 8) fetch(r);
-  uint4 rw[VPT];
+  uint4 rw[VPT];   // past the row's end 0
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = (tid + i * step) * V;
     rw[i] = make_uint4(0, 0, 0, 0);
     if (MODE == kRowsNorm && c < P.cols) rw[i] = load_raw<V>(P.weight, c);
   }
+  int parity = 0;
   for (; r < P.rows; r += stride) {
-    float v[VPT][V];
+    float2 v[VPT][H];
+    float2 ss = make_float2(0.0f, 0.0f);
+    float top = 0.0f;
     if constexpr (V == 8) cp_async_wait_all();
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -196,89 +242,73 @@ __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_quant_kernel(const
         rx = V == 8 ? mine[i * blockDim.x] : load_raw<V>(P.x, r * P.ldx + c);
         if (two) ro = V == 8 ? mine[(VPT + i) * blockDim.x] : load_raw<V>(other, r * ld_other + c);
       }
-      float o[V];
-      unpack_raw<DT, V>(rx, v[i]);
-      unpack_raw<DT, V>(ro, o);   // zeroes where there is no second input
+      const uint32_t wx[4] = {rx.x, rx.y, rx.z, rx.w}, wo[4] = {ro.x, ro.y, ro.z, ro.w};
+      const uint32_t ww[4] = {rw[i].x, rw[i].y, rw[i].z, rw[i].w};
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (MODE == kRowsSwiglu) v[i][j] = silu_of(v[i][j]) * o[j];
-        if (MODE == kRowsNorm) v[i][j] += o[j];
+      for (int j = 0; j < H; ++j) {
+        float2 a = unpack2<DT>(wx[j]);
+        if constexpr (MODE == kRowsSwiglu) a = mul2(make_float2(silu_of(a.x), silu_of(a.y)), unpack2<DT>(wo[j]));
+        if constexpr (MODE == kRowsNorm) {
+          if (two) a = add2(a, unpack2<DT>(wo[j]));
+          ss = fma2(a, a, ss);
+        }
+        v[i][j] = a;
+      }
+      if (MODE == kRowsNorm && P.residual_out != nullptr && c < P.cols) {
+        const long long o = r * P.ld_residual_out + c;
+        if constexpr (V == 8) {
+          __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(P.residual_out) + o),
+                 make_uint4(pack16<DT>(v[i][0].x, v[i][0].y), pack16<DT>(v[i][1].x, v[i][1].y),
+                            pack16<DT>(v[i][2].x, v[i][2].y), pack16<DT>(v[i][3].x, v[i][3].y)));
+        } else {
+          store16<DT>(P.residual_out, o, v[i][0].x);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        if constexpr (MODE == kRowsNorm) v[i][j] = mul2(v[i][j], unpack2<DT>(ww[j]));
+        top = max_abs(max_abs(top, v[i][j].x), v[i][j].y);
       }
     }
     if constexpr (V == 8)
       if (r + stride < P.rows) fetch(r + stride);
-    if constexpr (MODE == kRowsNorm) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int c = (tid + i * step) * V;
-        if (P.residual_out != nullptr && c < P.cols) {
-          const long long o = r * P.ld_residual_out + c;
-          if constexpr (V == 8) {
-            __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(P.residual_out) + o),
-                   make_uint4(pack16<DT>(v[i][0], v[i][1]), pack16<DT>(v[i][2], v[i][3]),
-                              pack16<DT>(v[i][4], v[i][5]), pack16<DT>(v[i][6], v[i][7])));
-          } else {
-            store16<DT>(P.residual_out, o, v[i][0]);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) ss += v[i][j] * v[i][j];
-      }
-      ss = __uint_as_float(row_reduce<ONE_WARP>(__float_as_uint(ss), sh[0], [](uint32_t a, uint32_t b) {
-        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
-      }));
-      const float rstd = rsqrtf(ss / static_cast<float>(P.cols) + P.eps);
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        float w[V];
-        unpack_raw<DT, V>(rw[i], w);
-        const bool in = (tid + i * step) * V < P.cols;   // past the end 0, even if rstd is not finite
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = in ? v[i][j] * rstd * w[j] : 0.0f;
-      }
-    }
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) top = max_abs(top, v[i][j]);
-    const uint32_t mx = row_reduce<ONE_WARP>(__float_as_uint(top), sh[1],
-                                             [](uint32_t a, uint32_t b) { return max(a, b); });
-    const RowScale s = row_scale<I8>(mx);
+    const RowStats st = row_reduce<ONE_WARP, MODE == kRowsNorm>(ss.x + ss.y, __float_as_uint(top), sh[parity]);
+    parity ^= 1;
+    const float gain = MODE == kRowsNorm ? rsqrtf(st.sum * P.inv_cols + P.eps) : 1.0f;
+    const RowScale s = row_scale<I8>(st.top, gain);
     if (tid == 0) P.scale[r] = s.scale;
     if (s.bad || s.lift != 1.0f) {   // rare, the same for the whole row
 #pragma unroll
       for (int i = 0; i < VPT; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = s.bad ? 0.0f : v[i][j] * s.lift;
+        for (int j = 0; j < H; ++j)
+          v[i][j] = s.bad ? make_float2(0.0f, 0.0f) : make_float2(v[i][j].x * s.lift, v[i][j].y * s.lift);
     }
+    const float2 inv = make_float2(s.inv, s.inv);
+    uint8_t* q = P.q + r * P.ldq;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = (tid + i * step) * V;
       if (c >= P.cols) continue;
+      uint32_t k[4];
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] *= s.inv;
-      uint8_t* q = P.q + r * P.ldq + c;
-      if constexpr (V == 8) {
-        __stcs(reinterpret_cast<uint2*>(q),
-               make_uint2(codes2<I8>(v[i][0], v[i][1]) | codes2<I8>(v[i][2], v[i][3]) << 16,
-                          codes2<I8>(v[i][4], v[i][5]) | codes2<I8>(v[i][6], v[i][7]) << 16));
-      } else {
-        q[0] = static_cast<uint8_t>(codes2<I8>(v[i][0], 0.0f));
+      for (int j = 0; j < H; ++j) {
+        const float2 a = mul2(v[i][j], inv);
+        k[j] = codes2<I8>(a.x, a.y);
       }
+      if constexpr (V == 8)
+        __stcs(reinterpret_cast<uint2*>(q + c), make_uint2(k[0] | k[1] << 16, k[2] | k[3] << 16));
+      else
+        q[c] = static_cast<uint8_t>(k[0]);
     }
-    // The norm's two barriers order the uses of sh between rows; the other
-    // modes have one a row and need a second before sh[1] is written again.
-    if constexpr (!ONE_WARP && MODE != kRowsNorm) __syncthreads();
   }
 }
 
-// Rows too long for the registers of one block: three passes over each, the
-// later ones from cache.
+// Rows too long for the registers of one block: two passes over each, the
+// second from cache.
 template <int DT, int MODE, int I8>
 __global__ void __launch_bounds__(1024) rows_quant_long_kernel(const RowsParams P) {
-  __shared__ uint32_t sh[2][32];
+  __shared__ uint2 sh[32];
   griddep_launch_dependents();
   griddep_wait();
   const long long r = blockIdx.x;
@@ -292,32 +322,21 @@ __global__ void __launch_bounds__(1024) rows_quant_long_kernel(const RowsParams 
       return v;
     }
   };
-  float rstd = 1.0f;
-  if constexpr (MODE == kRowsNorm) {
-    float ss = 0.0f;
-    for (int c = threadIdx.x; c < P.cols; c += blockDim.x) {
-      const float v = base(c);
-      ss += v * v;
-    }
-    ss = __uint_as_float(row_reduce<false>(__float_as_uint(ss), sh[0], [](uint32_t a, uint32_t b) {
-      return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
-    }));
-    rstd = rsqrtf(ss / static_cast<float>(P.cols) + P.eps);
+  auto weight = [&](int c) { return MODE == kRowsNorm ? load16<DT>(P.weight, c) : 1.0f; };
+  float ss = 0.0f, top = 0.0f;
+  for (int c = threadIdx.x; c < P.cols; c += blockDim.x) {
+    const float b = base(c);
+    ss += b * b;
+    top = max_abs(top, b * weight(c));
   }
-  auto value = [&](float b, int c) {
-    if constexpr (MODE == kRowsNorm) return b * rstd * load16<DT>(P.weight, c);
-    else return b;
-  };
-  uint32_t mx = 0;
-  for (int c = threadIdx.x; c < P.cols; c += blockDim.x)
-    mx = max(mx, __float_as_uint(value(base(c), c)) & 0x7FFFFFFFu);
-  mx = row_reduce<false>(mx, sh[1], [](uint32_t a, uint32_t b) { return max(a, b); });
-  const RowScale s = row_scale<I8>(mx);
+  const RowStats st = row_reduce<false, MODE == kRowsNorm>(ss, __float_as_uint(top), sh);
+  const RowScale s =
+      row_scale<I8>(st.top, MODE == kRowsNorm ? rsqrtf(st.sum * P.inv_cols + P.eps) : 1.0f);
   if (threadIdx.x == 0) P.scale[r] = s.scale;
   for (int c = threadIdx.x; c < P.cols; c += blockDim.x) {
     // The sum is written last: residual_out may be the residual itself.
     const float b = base(c);
-    const float v = s.bad ? 0.0f : value(b, c) * s.lift * s.inv;
+    const float v = s.bad ? 0.0f : b * weight(c) * s.lift * s.inv;
     if (MODE == kRowsNorm && P.residual_out != nullptr)
       store16<DT>(P.residual_out, r * P.ld_residual_out + c, b);
     P.q[r * P.ldq + c] = static_cast<uint8_t>(codes2<I8>(v, 0.0f));

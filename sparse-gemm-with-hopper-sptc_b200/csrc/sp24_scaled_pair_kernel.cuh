@@ -100,20 +100,6 @@ SP24_DEV void scaled_tile(const ScaledPairParams& P, int t, int& mt, int& nt) {
   nt = r / gm;
 }
 
-// Two fp32 operations in one instruction.
-SP24_DEV float2 mul2(float2 a, float2 b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
-  return *reinterpret_cast<float2*>(&r);
-}
-SP24_DEV float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(r)
-      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
-  return *reinterpret_cast<float2*>(&r);
-}
-
 template <int I8>
 SP24_DEV float sum_value(uint32_t a) {
   return I8 ? static_cast<float>(static_cast<int>(a)) : __uint_as_float(a);
