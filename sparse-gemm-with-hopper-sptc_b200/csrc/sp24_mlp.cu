@@ -347,9 +347,15 @@ sp24_status scaled_pair(const FfnCall& c, const sp24_scaled_desc* d) {
   p.status = c.status;
   p.timeout_ns = kDefaultTimeoutNs;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
-  if (tiles > 0x7fffffff / 2) return SP24_ERR_SHAPE;
-  const unsigned pairs = static_cast<unsigned>(std::min<long long>(tiles, c.sm_count / 2));
-  return launch_gemm_kernel(kern, 2 * pairs, sp24::kScaledThreads, C::SMEM_BYTES, c.stream, 0, true, a, b, e, p);
+  if (tiles > 0x7fffffff / 4) return SP24_ERR_SHAPE;
+  // A last wave that half the pairs could cover is dealt block by block.
+  const int pairs = c.sm_count / 2;
+  const int last = static_cast<int>(tiles % pairs);
+  const bool halve = MB == 2 && 2 * last <= pairs;
+  p.whole_items = static_cast<int>(halve ? tiles - last : tiles);
+  p.items = p.whole_items + (halve ? 2 * last : 0);
+  return launch_gemm_kernel(kern, static_cast<unsigned>(2 * std::min(p.items, pairs)), sp24::kScaledThreads,
+                            C::SMEM_BYTES, c.stream, 0, true, a, b, e, p);
 }
 
 // Which kernel.  Up to 32 tokens the weights' bytes decide, and the streaming
@@ -358,19 +364,23 @@ sp24_status scaled_pair(const FfnCall& c, const sp24_scaled_desc* d) {
 // three quarters of the pairs (14336 x 4096, 64 / 128 tokens: 13.7 / 13.9 us
 // against 15.0 / 21.8; 4096 x 14336 has 16 such tiles: 28 us against 13 / 17).
 // Beyond, tiles of one 256-row block x 128 tokens fill few waves, and tiles of
-// two blocks x 224 tokens load less per product: one wave of the large tile
-// costs 2.6 of the small one (K = 4096: 17.5 and 6.7 us), so it is taken where
-// it saves more waves than that (14336 x 4096: 200 tokens 26.3 against 20.1 us
-// on the small tile, 1024 tokens 41.6 against 55.0).
+// two blocks x 224 tokens load less per product: a wave of the large tile takes
+// twice as long as one of the small (K = 14336: 47 and 25 us; K = 4096: 18 and 8),
+// and its last wave may go in halves.  The large tile is taken where it ends
+// sooner (4096 tokens x 4096 x 14336: 2.5 large waves or 7 small, 137 and 178 us;
+// 1024 tokens x 14336 x 4096: 2 or 7, 40.6 and 53.4 us; 333 x 5003 x 4160: half a
+// wave or one, 16.3 and 12.4 us, and a tie goes to the small).
 template <int I8>
 sp24_status scaled(const FfnCall& c, const sp24_scaled_desc* d) {
   const long long pairs = c.sm_count / 2;
   const long long blocks = (d->m + 255) / 256;
   if (d->n <= 32 || (d->n <= kStreamMaxTokens && 4 * blocks < 3 * pairs)) return scaled_few<I8>(c, d);
-  auto waves = [&](long long tiles) { return (tiles + pairs - 1) / pairs; };
-  const long long small = waves(blocks * ((d->n + 127) / 128));
-  const long long large = waves((d->m + 511LL) / 512 * ((d->n + 223LL) / 224));
-  return 10 * small > 26 * large ? scaled_pair<I8, 2, 224>(c, d) : scaled_pair<I8, 1, 128>(c, d);
+  const long long small_tiles = blocks * ((d->n + 127LL) / 128);
+  const long long large_tiles = (d->m + 511LL) / 512 * ((d->n + 223LL) / 224);
+  const long long small = (small_tiles + pairs - 1) / pairs;
+  const long long last = large_tiles % pairs;
+  const long long halves = large_tiles / pairs * 2 + (last == 0 ? 0 : 2 * last <= pairs ? 1 : 2);
+  return small > halves ? scaled_pair<I8, 2, 224>(c, d) : scaled_pair<I8, 1, 128>(c, d);
 }
 
 template <int DT>

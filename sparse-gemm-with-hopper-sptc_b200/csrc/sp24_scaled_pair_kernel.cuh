@@ -9,19 +9,24 @@
 // and compressed weights are the cheaper operand (half the values, plus an eighth
 // for the codes).
 //   MB = 2, BN = 224  two blocks of 256 weight rows against one staged block of
-//                     tokens: 68 KB per 1273 clocks of MMAs and 256 of K.  The
-//                     accumulators take 2 x 224 TMEM columns and the
-//                     double-buffered metadata 2 x 16 of the rest, so they are
-//                     single-buffered; the epilogue hands each back once its
-//                     columns are in registers.
-//   MB = 1, BN = 128  36 KB per 364 clocks: more loading per product, but twice
+//                     tokens: 68 KB per 1270 clocks of MMAs and 256 of K.  The
+//                     accumulators take 2 x 224 TMEM columns and the metadata
+//                     buffers most of the rest, so they are single-buffered;
+//                     the epilogue hands each back once its columns are in
+//                     registers.  A last wave that would fill at most half the
+//                     pairs is dealt block by block.
+//   MB = 1, BN = 128  36 KB per 360 clocks: more loading per product, but twice
 //                     as many tiles in both directions and two accumulator
 //                     buffers, for calls that do not fill the GPU with the other.
-// 14336 x 4096 int8, 4096 tokens (481 dense-equivalent GFLOP): 143 us, of which the
-// MMAs alone would take about 96 at the 1.7 GHz the power cap leaves; without its
-// stores the kernel takes 115, without its MMAs 114.  The layout of the stores
-// does not matter (full 128-byte lines: 144), nor do 128-deep stages in a ring
-// twice as long (their 64-byte weight rows load slower: 188).
+// 14336 x 4096 int8, 4096 tokens (481 dense-equivalent GFLOP): 134 us in a burst,
+// 145 held under the 1000 W cap at 1.69 GHz, where the MMAs alone would take 86.
+// Shared memory bounds the main loop (per stage and SM the MMAs read 88 KB and
+// the copies write 68, 97 bytes a clock together): without its stores the
+// kernel takes 115 us, without its MMAs 114.  Measured and not kept: 128-byte
+// store lines (144 against 144), cache policies on weights or output (the same),
+// both accumulators packed before the first store (164), starting block 0 while
+// block 1 drains (148; with three stages ahead 147), 128-deep stages in a ring
+// twice as long (188: their 64-byte weight rows load slower).
 //
 // Accumulator lanes are weight rows, i.e. neighbouring features of a token's
 // output row: a warp's store of one token is one contiguous 64-byte run.
@@ -42,6 +47,8 @@ constexpr int kScaledAWarp = 8, kScaledMmaWarp = 9, kScaledBWarp = 10;
 struct ScaledPairParams {
   int m, n, k;
   int m_tiles, n_tiles, k_stages;
+  int items;          // units of work: whole tiles, then
+  int whole_items;    // single blocks of the tiles from whole_items on (MB = 2)
   int group_m;
   int meta_mblocks;
   const float *scale_m, *scale_n, *bias;
@@ -70,13 +77,13 @@ struct ScaledPairCfg {
   static constexpr int STAGES_RAW = (kSmemBudget - 5 * 1024) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
-  // TMEM: accumulator b at column 256 b, metadata buffer e after accumulator e.
+  // TMEM: accumulator b at column 256 b, two of four metadata buffers after each.
   static constexpr int E_COL = BN;
   static constexpr uint32_t IDESC =
       I8 ? ((1u << 2) | (2u << 4) | (1u << 7) | (1u << 10) | ((BN >> 3) << 17) | ((256u >> 4) << 24))
          : make_idesc_sparse(0, BN, 256, false);
   static constexpr int CW = BN / 2;                     // columns per epilogue warp
-  static_assert(BN % 32 == 0 && BN + MB * ATOMS * 4 <= 256, "tokens per tile");
+  static_assert(BN % 32 == 0 && BN + 2 * MB * ATOMS * 4 <= 256, "tokens per tile");
   static_assert(B_BOX % 1024 == 0 && STAGE_BYTES % 1024 == 0, "boxes stay 1024-aligned");
   static_assert(STAGES >= 3, "ring");
 };
@@ -90,14 +97,19 @@ SP24_DEV void tc_mma_sp_pair_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t e, 
       : "memory");
 }
 
-SP24_DEV void scaled_tile(const ScaledPairParams& P, int t, int& mt, int& nt) {
+// Unit of work `it`: tile column nt, `blocks` blocks of 256 weight rows from `block`.
+template <int MB>
+SP24_DEV void scaled_item(const ScaledPairParams& P, int it, int& nt, int& block, int& blocks) {
+  const int half = it - P.whole_items;
+  const int t = half < 0 ? it : P.whole_items + half / MB;
   const int per_group = P.group_m * P.n_tiles;
   const int g = t / per_group;
   const int first = g * P.group_m;
   const int gm = min(P.m_tiles - first, P.group_m);
   const int r = t - g * per_group;
-  mt = first + r % gm;
   nt = r / gm;
+  block = (first + r % gm) * MB + (half < 0 ? 0 : half % MB);
+  blocks = half < 0 ? MB : 1;
 }
 
 template <int I8>
@@ -182,8 +194,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kScaledThreads, 1)
   const bool leader = prank == 0;
   const int pair = static_cast<int>(blockIdx.x >> 1);
   const int npairs = static_cast<int>(gridDim.x >> 1);
-  const int num_tiles = P.m_tiles * P.n_tiles;
   const uint64_t tmo = P.timeout_ns;
+  // Bytes of both CTAs for the stage `ahead` of the first stage of unit `it`.
+  auto stage_tx = [&](int it, int ahead) {
+    if (ahead >= P.k_stages) it += ahead / P.k_stages * npairs;
+    const int blocks = it < P.whole_items ? MB : 1;
+    return static_cast<uint32_t>(2 * (blocks * (C::A_BOX + C::ATOMS * kAtomBytes) + C::B_BYTES));
+  };
 
   if (threadIdx.x == 0) {
     abort_sh = 0;
@@ -198,7 +215,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kScaledThreads, 1)
     // Armed here for the first use, by the MMA warp for later ones; both CTAs'
     // bytes land on the leader's barriers (TMA counts zero-filled ones too).
     if (leader)
-      for (int s = 0; s < C::STAGES; ++s) mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
+      for (int s = 0; s < C::STAGES; ++s) mbar_arrive_expect_tx(&full_bar[s], stage_tx(pair, s));
   }
   if (warp == kScaledAWarp && lane == 0) {
     tma_prefetch_desc(&tmA);
@@ -223,7 +240,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kScaledThreads, 1)
     if (is_b || !P.static_weights) griddep_wait();
     const bool is_a = !is_b && lane < MB;
     const int el = lane - MB;                           // block el / ATOMS, its atom el % ATOMS
-    const int lanes = is_b ? C::B_BOXES : MB + MB * C::ATOMS;
     const CUtensorMap* map = is_b ? &tmB : is_a ? &tmA : &tmE;
     const uint32_t off = is_b   ? C::A_BYTES + lane * C::B_BOX
                          : is_a ? lane * C::A_BOX
@@ -235,17 +251,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kScaledThreads, 1)
     uint32_t ph = 0;
     bool ok = true;
     uint32_t used_mask = 0, used_ph = 0;
-    for (int t = pair; t < num_tiles && ok; t += npairs) {
-      int mt, nt;
-      scaled_tile(P, t, mt, nt);
+    for (int it = pair; it < P.items && ok; it += npairs) {
+      int nt, block, blocks;
+      scaled_item<MB>(P, it, nt, block, blocks);
       int x = is_b ? lane * 128 : 0, y;
+      bool loads;
       if (is_b) {
+        loads = lane < C::B_BOXES;
         y = nt * BN + prank * C::HALF;
       } else if (is_a) {
-        y = (mt * MB + lane) * 256 + prank * 128;
+        loads = lane < blocks;
+        y = (block + lane) * 256 + prank * 128;
       } else {
+        loads = el < blocks * C::ATOMS;
         // Blocks past the image belong to rows past m: any valid codes serve.
-        const int mb = min((mt * MB + el / C::ATOMS) * 2 + prank, P.meta_mblocks - 1);
+        const int mb = min((block + el / C::ATOMS) * 2 + prank, P.meta_mblocks - 1);
         y = ((el % C::ATOMS) * P.meta_mblocks + mb) * 8;
       }
       for (int ks = 0; ks < P.k_stages; ++ks) {
@@ -259,7 +279,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kScaledThreads, 1)
           used_mask |= 1u << s;
           used_ph = (used_ph & ~(1u << s)) | (ph << s);
         }
-        if (lane < lanes)
+        if (loads)
           tma_load_2d_pair(smem + s * C::STAGE_BYTES + off, map, full0 + s * sizeof(uint64_t), x, y);
         x += dx;
         y += dy;
@@ -280,52 +300,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kScaledThreads, 1)
       const uint64_t bdesc0 = make_sdesc(base + C::A_BYTES, 16, 1024, kLayoutSW128);
       const uint64_t edesc0 = make_sdesc(base + C::A_BYTES + C::B_BYTES, kAtomBytes, 128, kLayoutNone);
       int s = 0;
-      uint32_t ph = 0, aph = 0, ebuf = 0, acc0 = 0;   // acc0: this tile's first accumulator
+      uint32_t ph = 0, aph = 0, eb = 0, acc0 = 0;   // acc0: this unit's first accumulator
       bool ok = true, any = false;
-      for (int t = pair; t < num_tiles && ok; t += npairs) {
-        int mt, nt;
-        scaled_tile(P, t, mt, nt);
-        for (int ks = 0; ks < P.k_stages && ok; ++ks) {
+      for (int it = pair; it < P.items && ok; it += npairs) {
+        int nt, block, blocks;
+        scaled_item<MB>(P, it, nt, block, blocks);
+        // Block b of a stage: its products, once the metadata is on its way.
+        auto products = [&](int ks, uint32_t e, int b) {
+          const int kleft = P.k - ks * C::BKD;
+          const uint64_t so = static_cast<uint64_t>(s * (C::STAGE_BYTES >> 4));
+          if ((block + b) * 256 < P.m && elect_one()) {
+#pragma unroll
+            for (int j = 0; j < C::MMAS; ++j)
+              if (j * 64 < kleft) {   // past K there is no metadata
+                const uint64_t ad = adesc0 + so + b * (C::A_BOX >> 4) + j * 2;
+                const uint64_t bd = bdesc0 + so + (j >> 1) * (C::B_BOX >> 4) + (j & 1) * 4;
+                const uint32_t d = tmem_base + (acc0 + b) * 256, ec = e + b * C::ATOMS * 4 + j * 2;
+                const uint32_t acc = (ks > 0 || j > 0) ? 1u : 0u;
+                if constexpr (I8) tc_mma_sp_pair_i8(d, ad, bd, ec, C::IDESC, acc);
+                else tc_mma_sp_pair<1>(d, ad, bd, ec, C::IDESC, acc);
+              }
+          }
+          __syncwarp();
+        };
+        // The last unit's columns of these accumulators are in registers.
+        for (int b = 0; b < blocks && ok; ++b) ok = mbar_wait_warp<true>(&acce_bar[acc0 + b], aph ^ 1u, &abort_sh, tmo);
+        if (!ok) break;
+        tc_fence_after();
+        for (int ks = 0; ks < P.k_stages; ++ks) {
           if (!mbar_wait_warp(&full_bar[s], ph, &abort_sh, tmo)) {
             ok = false;
             break;
           }
-          if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
           tc_fence_after();
-          ebuf ^= 1u;
-          const uint32_t e = tmem_base + ebuf * 256 + C::E_COL;
-          const int kleft = P.k - ks * C::BKD;
-          const uint64_t so = static_cast<uint64_t>(s * (C::STAGE_BYTES >> 4));
+          const uint32_t e = tmem_base + (eb & 1u) * 256 + C::E_COL + (eb >> 1 & 1u) * (MB * C::ATOMS * 4);
+          ++eb;
           if (elect_one()) {
+            const uint64_t ed = edesc0 + static_cast<uint64_t>(s * (C::STAGE_BYTES >> 4));
 #pragma unroll
-            for (int a = 0; a < MB * C::ATOMS; ++a) tc_cp<2>(e + 4 * a, edesc0 + so + a * (kAtomBytes >> 4));
+            for (int a = 0; a < MB * C::ATOMS; ++a)
+              if (a < blocks * C::ATOMS) tc_cp<2>(e + 4 * a, ed + a * (kAtomBytes >> 4));
           }
           __syncwarp();
-#pragma unroll
-          for (int b = 0; b < MB; ++b) {
-            if (ks == 0) {   // this accumulator's columns of the last tile are in registers
-              if (!mbar_wait_warp<true>(&acce_bar[acc0 + b], aph ^ 1u, &abort_sh, tmo)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-            }
-            if ((mt * MB + b) * 256 < P.m && elect_one()) {
-#pragma unroll
-              for (int j = 0; j < C::MMAS; ++j)
-                if (j * 64 < kleft) {   // past K there is no metadata
-                  const uint64_t ad = adesc0 + so + b * (C::A_BOX >> 4) + j * 2;
-                  const uint64_t bd = bdesc0 + so + (j >> 1) * (C::B_BOX >> 4) + (j & 1) * 4;
-                  const uint32_t d = tmem_base + (acc0 + b) * 256, ec = e + b * C::ATOMS * 4 + j * 2;
-                  const uint32_t acc = (ks > 0 || j > 0) ? 1u : 0u;
-                  if constexpr (I8) tc_mma_sp_pair_i8(d, ad, bd, ec, C::IDESC, acc);
-                  else tc_mma_sp_pair<1>(d, ad, bd, ec, C::IDESC, acc);
-                }
-            }
-            __syncwarp();
-            any = true;
-          }
-          if (!ok) break;
+          any = true;
+          products(ks, e, 0);
+          if (blocks == 2) products(ks, e, 1);
+          // Armed for the slot's next use only now, off the products' path; freed
+          // once they are done.
+          if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], stage_tx(it, ks + C::STAGES));
+          __syncwarp();
           if (elect_one()) tc_commit_pair(&empty_bar[s], 3);
           __syncwarp();
           if (++s == C::STAGES) s = 0, ph ^= 1u;
@@ -351,9 +374,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kScaledThreads, 1)
     const uint32_t acce0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
     uint32_t aph = 0, acc0 = 0;
     griddep_wait();   // scales and bias may come from the previous kernel
-    for (int t = pair; t < num_tiles; t += npairs) {
-      int mt, nt;
-      scaled_tile(P, t, mt, nt);
+    for (int it = pair; it < P.items; it += npairs) {
+      int nt, block, blocks;
+      scaled_item<MB>(P, it, nt, block, blocks);
       float* sn = sn_sh[warp];
       __syncwarp();
       for (int j = lane; j < C::CW; j += 32) {
@@ -368,6 +391,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kScaledThreads, 1)
       const int t0 = nt * BN + half * C::CW;
 #pragma unroll 1
       for (int b = 0; b < MB; ++b) {
+        const int row = (block + b) * 256 + prank * 128 + q * 32 + lane;
+        if (b >= blocks) {
+          if (lane == 0) mbar_arrive_cluster(acce0 + (acc0 + b) * sizeof(uint64_t));
+          continue;
+        }
         uint32_t r[C::CW];
         const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
                             (acc0 + b) * 256 + half * C::CW;
@@ -377,7 +405,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kScaledThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(acce0 + (acc0 + b) * sizeof(uint64_t));
-        const int row = (mt * MB + b) * 256 + prank * 128 + q * 32 + lane;
         if (row - lane >= P.m) continue;
         if (P.out_type == 2) scaled_emit<I8, C::CW, 2>(P, r, row, t0, sn);
         else if (P.out_type == 1) scaled_emit<I8, C::CW, 1>(P, r, row, t0, sn);
