@@ -165,7 +165,7 @@ sp24_status sp24_gemm(const sp24_gemm_desc* d, sp24_stream_t stream);
 sp24_status sp24_last_kernel_status(sp24_stream_t stream);
 
 /* Launch hints for later GEMM calls made from the calling host thread (no
-   reference counterpart).  GEMM kernels are launched with programmatic
+   reference counterpart; sp24_gemm_scaled and sp24_ffn_forward take them too).  GEMM kernels are launched with programmatic
    dependent launch: they may start while the previous kernel of the stream
    finishes and wait for it before their first load.
    SP24_HINT_STATIC_WEIGHTS: the caller guarantees that A_c and the metadata

@@ -212,8 +212,8 @@ sp24_status launch_ffn_pair(const FfnCall& c, const CUtensorMap (&a)[2], const C
 // The largest number of K splits, at most `want`, whose clusters (`per_split`
 // CTAs each) are all resident at once: a second wave of clusters would cost
 // more than the split saves.
-template <typename Kern>
-int resident_splits(Kern kern, int threads, int smem, long long clusters, int per_split, int want) {
+template <auto Kern>
+int resident_splits(int threads, int smem, long long clusters, int per_split, int want) {
   static std::atomic<int> cache[kMaxDevices][9];   // by CTAs per cluster; 0 = not asked yet
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 1;
@@ -231,7 +231,7 @@ int resident_splits(Kern kern, int threads, int smem, long long clusters, int pe
       attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+      if (cudaOccupancyMaxActiveClusters(&n, Kern, &cfg) != cudaSuccess) {
         (void)cudaGetLastError();
         n = 0;
       }
@@ -266,7 +266,7 @@ sp24_status launch_stream_bn(const FfnCall& c, const CUtensorMap& a, const CUten
   const long long tiles = static_cast<long long>(p.m_blocks) * n_tiles;
   if (tiles * sp24::kStreamMaxSplits > 0x7fffffff) return SP24_ERR_SHAPE;
   const int want = static_cast<int>(std::min<long long>({c.sm_count / tiles, sp24::kStreamMaxSplits, p.stages}));
-  p.splits = resident_splits(kern, sp24::kStreamThreads, C::SMEM_BYTES, tiles, 1, want);
+  p.splits = resident_splits<sp24::stream_kernel<OP, BN>>(sp24::kStreamThreads, C::SMEM_BYTES, tiles, 1, want);
   // No more slots than a CTA has stages: what is left of the SM's shared memory
   // lets the next kernel's CTAs start their prologue beside this one's tail
   // (4096 x 4096, 1 token, back to back: 6.1 -> 5.6 us).
@@ -438,7 +438,7 @@ int dx_splits(long long tiles, int want) {
   static std::atomic<bool> attr_set[kMaxDevices];
   auto kern = sp24::ffn_dx_split_kernel<DT>;
   if (ensure_kernel_attrs(kern, attr_set, smem) != SP24_OK) return 1;
-  return resident_splits(kern, sp24::kPairThreads, smem, tiles, 2, want);
+  return resident_splits<sp24::ffn_dx_split_kernel<DT>>(sp24::kPairThreads, smem, tiles, 2, want);
 }
 
 template <int DT>
