@@ -5,7 +5,7 @@
 //   c[t][r]   = acc * scale_m[r] * scale_n[t] + bias[r]    N = BN, K = 64 per MMA
 //
 // Two tiles.  The tensor pipe takes about 11.6k multiply-adds a clock and SM of
-// this kind, an SM takes in about 64 bytes a clock (profiles/sp24_feed_probe.md),
+// this kind, an SM takes in about 64 bytes a clock (bin/sp24_feed_probe),
 // and compressed weights are the cheaper operand (half the values, plus an eighth
 // for the codes).
 //   MB = 2, BN = 224  two blocks of 256 weight rows against one staged block of

@@ -407,4 +407,195 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #endif
 }
 
+// The gated block over 33 to 128 tokens, still bound by the weights' bytes: a CTA
+// pair takes 256 rows of Wg and the same 256 of Wu as the M of two MMAs
+// (tcgen05.mma.cta_group::2, M = 256, N = BN) against one staged block of tokens,
+// of which each CTA loads half.  Staging half the tokens leaves the ring to the
+// weights: at 128 tokens 32 of a stage's 40 KB, where a single CTA's stages hold
+// 32 of 48 (4096 -> 14336 bf16, 128 tokens: 48.2 us against 57.6).  Both
+// accumulators of a feature lie in one lane, at columns 0 and 256.
+template <int BN>
+struct FewPairCfg {
+  static constexpr int BK = 64;
+  static constexpr int A_BOX = kBlockM * 128;
+  static constexpr int A_BYTES = 2 * A_BOX;             // Wg's rows, then Wu's
+  static constexpr int HALF = BN / 2;                   // tokens staged per CTA
+  static constexpr int B_BYTES = HALF * 128;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES_RAW = (kSmemBudget - 1024) / STAGE_BYTES;
+  static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
+  static constexpr int CW = BN / 2;                     // columns per epilogue warp
+  static_assert(BN % 64 == 0 && BN <= 128 && STAGE_BYTES % 1024 == 0, "token tile");
+};
+
+// tmA, tmA2: Wg and Wu; tmB: the tokens.  One pair per 256 features.
+template <int DT, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    few_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA2,
+                    const __grid_constant__ CUtensorMap tmB, const StreamParams P) {
+#if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
+  using C = FewPairCfg<BN>;
+  constexpr uint32_t IDESC = make_idesc_dense(DT, BN, 256, false, false);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t accf_bar;
+  __shared__ __align__(8) uint64_t drain_bar;
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ volatile int abort_sh;
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int prank = static_cast<int>(cluster_ctarank());
+  const bool leader = prank == 0;
+  const int row_cta = static_cast<int>(blockIdx.x >> 1) * 256 + prank * 128;   // this CTA's first feature
+  const uint64_t tmo = P.timeout_ns;
+
+  if (threadIdx.x == 0) {
+    abort_sh = 0;
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&accf_bar, 1);
+    mbar_init(&drain_bar, 1);
+    fence_barrier_init();
+    // Both CTAs' bytes land on the leader's barriers, armed here for the first
+    // use and by the MMA warp for later ones.
+    if (leader)
+      for (int s = 0; s < C::STAGES; ++s) mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmA2);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&tmem_base_sh, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_sh;
+  griddep_launch_dependents();
+
+  if (warp == 0 || warp == kPairBWarp) {
+    // ------------------------------------------------------------ producers
+    const bool is_b = warp == kPairBWarp;
+    if (is_b || !P.static_weights) griddep_wait();
+    const CUtensorMap* map = is_b ? &tmB : lane == 1 ? &tmA2 : &tmA;
+    const uint32_t off = is_b ? C::A_BYTES : lane * C::A_BOX;
+    const int y = is_b ? prank * C::HALF : row_cta;
+    const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);
+    int s = 0;
+    uint32_t ph = 0, used_mask = 0, used_ph = 0;
+    bool ok = true;
+    for (int ks = 0; ks < P.stages; ++ks) {
+      int good = 1;
+      if (lane == 0) good = mbar_wait_fast(&empty_bar[s], ph ^ 1u, &abort_sh, tmo) ? 1 : 0;
+      if (__shfl_sync(0xffffffffu, good, 0) == 0) {
+        ok = false;
+        break;
+      }
+      used_mask |= 1u << s;
+      used_ph = (used_ph & ~(1u << s)) | (ph << s);
+      if (lane < (is_b ? 1 : 2))
+        tma_load_2d_pair(smem + s * C::STAGE_BYTES + off, map, full0 + s * sizeof(uint64_t), ks * C::BK, y);
+      if (++s == C::STAGES) s = 0, ph ^= 1u;
+    }
+    if (!ok && leader && lane == 0) {
+      // Error path: copies in flight land before the CTA leaves.
+      volatile int dummy = 0;
+      for (int i = 0; i < C::STAGES; ++i)
+        if (used_mask & (1u << i)) mbar_wait(&full_bar[i], (used_ph >> i) & 1u, &dummy, tmo);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader)
+    if (leader) {
+      const uint32_t base = smem_u32(smem);
+      const uint64_t adesc0 = make_sdesc(base, 16, 1024, kLayoutSW128);
+      const uint64_t bdesc0 = make_sdesc(base + C::A_BYTES, 16, 1024, kLayoutSW128);
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true, any = false;
+      for (int ks = 0; ks < P.stages; ++ks) {
+        if (!mbar_wait_warp(&full_bar[s], ph, &abort_sh, tmo)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t so = static_cast<uint64_t>(s * (C::STAGE_BYTES >> 4));
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int j = 0; j < C::BK / 16; ++j)
+              tc_mma_dense_pair(tmem_base + w * 256, adesc0 + so + w * (C::A_BOX >> 4) + j * 2,
+                                bdesc0 + so + j * 2, IDESC, (ks > 0 || j > 0) ? 1u : 0u);
+          tc_commit_pair(&empty_bar[s], 3);
+        }
+        __syncwarp();
+        any = true;
+        if (++s == C::STAGES) s = 0, ph ^= 1u;
+      }
+      if (ok && elect_one()) tc_commit_pair(&accf_bar, 3);
+      __syncwarp();
+      if (!ok && any) {
+        volatile int dummy = 0;
+        if (elect_one()) tc_commit_pair(&drain_bar, 1);
+        __syncwarp();
+        if (lane == 0) mbar_wait(&drain_bar, 0, &dummy, tmo);
+        __syncwarp();
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    bool ok = true;
+    if (lane == 0) ok = mbar_wait_sleepy(&accf_bar, 0, &abort_sh, tmo);
+    if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0) {
+      tc_fence_after();
+      const int row = row_cta + q * 32 + lane;
+      const int t0 = half * C::CW, t1 = min(P.n, t0 + C::CW);
+      const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+#pragma unroll 1
+      for (int t = t0; t < t1; t += 16) {
+        uint32_t g[16], u[16];
+        tmem_ld_x16(tb + t, g);
+        tmem_ld_x16(tb + 256 + t, u);
+        tmem_ld_wait(g);
+        tmem_ld_wait(u);
+        if (row >= P.m) continue;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const long long tok = t + j;
+          if (tok < t1) {
+            if (P.saved != nullptr) {
+              P.saved[tok * P.ld_saved + row] = __uint_as_float(g[j]);
+              P.saved[(P.n + tok) * P.ld_saved + row] = __uint_as_float(u[j]);
+            }
+            store16<DT>(P.out, tok * P.ldo + row,
+                        gate_act(__uint_as_float(g[j]), P.silu) * __uint_as_float(u[j]));
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+  if (threadIdx.x == 0 && abort_sh != 0 && P.status != nullptr) atomicExch(P.status, 1);
+#endif
+}
+
 }  // namespace sp24

@@ -373,7 +373,8 @@ def check_ffn(x, wg, wu, dh, act, out, grads=None):
                                    (16, 4096, 640), (17, 200, 200), (31, 512, 72), (33, 64, 2744), (64, 1024, 256),
                                    (65, 128, 128), (100, 264, 1032), (128, 256, 256), (129, 512, 136), (257, 320, 512),
                                    (300, 1000, 776), (513, 256, 1024),
-                                   (1300, 1280, 264), (1030, 1000, 136), (2600, 264, 512)])
+                                   (1300, 1280, 264), (1030, 1000, 136), (2600, 264, 512),
+                                   (33, 72, 14336), (100, 264, 15000), (129, 200, 18888), (256, 64, 16384)])
 def test_ffn_sizes(t, h, f, dtype, act):
     x, wg, wu, dh = ffn_inputs(t, h, f, dtype, seed=t + h)
     out, saved = sp24.ffn_gated(x, wg, wu, act=act, save=True)
@@ -542,3 +543,65 @@ def test_shim_refuses_wrong_types_and_shapes():
         sp24.gemm_scaled(i8(128, 16), image[:2 * 2048], i8(4, 32))
     with pytest.raises(sp24.Sp24Error):      # a saved buffer of another call
         sp24.ffn_gated_backward(bf(4, 96), bf(4, 64), bf(96, 64), bf(96, 64), image[:64])
+
+
+def test_static_weight_hint_and_graphs_keep_results():
+    """SP24_HINT_STATIC_WEIGHTS only moves weight loads ahead of the wait for the
+    previous kernel; a captured call replays on new inputs.  The tokens are
+    written by the kernel just before each product."""
+    a_c, image, w = weights_2of4(512, 1024, sp24.I8, seed=1)
+    wg, wu = (randn(512, 1024, seed=s, std=0.02, dtype=torch.bfloat16) for s in (2, 3))
+    for n in (1, 40, 300):
+        xs = [randn(n, 1024, seed=10 + i, dtype=torch.bfloat16) for i in range(3)]
+
+        def chain(x):
+            q, s = sp24.quantize_rows(x)
+            return sp24.gemm_scaled(a_c, image, q, None, s, out_dtype=torch.float32), sp24.ffn_gated(x, wg, wu)
+
+        want = [chain(x) for x in xs]
+        sp24.set_launch_hints(sp24.HINT_STATIC_WEIGHTS)
+        try:
+            got = [chain(x) for x in xs]
+        finally:
+            sp24.set_launch_hints(sp24.HINT_NONE)
+        assert all(torch.equal(a, b) for p, q in zip(got, want) for a, b in zip(p, q))
+        x = xs[0].clone()
+        side = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(graph, stream=side):
+            out = chain(x)
+        for i in (1, 2):
+            x.copy_(xs[i])
+            graph.replay()
+            assert torch.equal(out[0], want[i][0]) and torch.equal(out[1], want[i][1])
+
+
+def test_calls_from_several_threads():
+    """First calls on a device may come from several host threads at once, each
+    on its own stream: results as from one."""
+    import threading
+    a_c, image, _ = weights_2of4(640, 512, sp24.E4M3, seed=1)
+    wg, wu = (randn(384, 512, seed=s, std=0.02, dtype=torch.float16) for s in (2, 3))
+    xs = [randn(n, 512, seed=n, dtype=torch.float16) for n in (1, 70, 200, 400)]
+
+    def work(x, stream=None):
+        q, s = sp24.quantize_rows(x, qdtype=sp24.E4M3, stream=stream)
+        return sp24.gemm_scaled(a_c, image, q, None, s, stream=stream), sp24.ffn_gated(x, wg, wu, stream=stream)
+
+    want = [work(x) for x in xs]
+    torch.cuda.synchronize()
+    got = [None] * len(xs)
+
+    def run(i):
+        stream = torch.cuda.Stream()
+        for _ in range(20):
+            got[i] = work(xs[i], stream)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for p, q in zip(got, want) for a, b in zip(p, q))
