@@ -34,6 +34,7 @@
 namespace sp24 {
 
 enum : int { kFfnForward = 0, kFfnDx = 1, kFfnDw = 2 };
+constexpr int kMaxDxSplits = 4;   // pairs per cluster of the K-split dx: 8 CTAs
 
 struct FfnParams {
   int m, n;                // rows of a plane's output, output columns (forward: f)
@@ -414,11 +415,14 @@ SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, co
     for (int i = threadIdx.x; i < rows * 64; i += kPairThreads) {
       const int rl = r0 + (i >> 6), cl = (i & 63) * 4;
       const uint32_t la = smem_u32(red + rl * C::RS + cl);
-      float4 a = ld_dsmem_f4(mapa_shared(la, static_cast<uint32_t>(prank)));
-      for (int sp = 1; sp < S; ++sp) {
-        const float4 v = ld_dsmem_f4(mapa_shared(la, static_cast<uint32_t>(2 * sp + prank)));
-        a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
-      }
+      float4 v[kMaxDxSplits];   // all loads on their way before the first sum
+#pragma unroll
+      for (int sp = 0; sp < kMaxDxSplits; ++sp)
+        if (sp < S) v[sp] = ld_dsmem_f4(mapa_shared(la, static_cast<uint32_t>(2 * sp + prank)));
+      float4 a = v[0];
+#pragma unroll
+      for (int sp = 1; sp < kMaxDxSplits; ++sp)
+        if (sp < S) a.x += v[sp].x, a.y += v[sp].y, a.z += v[sp].z, a.w += v[sp].w;
       const int row = mt * 256 + prank * 128 + rl, col = nt * 256 + cl;
       if (row >= P.m) continue;
       uint16_t* dst = static_cast<uint16_t*>(P.out0) + row * P.ld_out0 + col;

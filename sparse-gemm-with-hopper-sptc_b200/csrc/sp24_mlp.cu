@@ -505,7 +505,7 @@ sp24_status ffn_backward(const FfnCall& c, const sp24_ffn_desc* d, const sp24_ff
     // Few tiles: K split over the pairs of a cluster (777 x 1000, f = 2744, 16
     // tiles of 86 stages: 48.3 -> 27.8 us with four, dg and du included).
     const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
-    const int want = static_cast<int>(std::min<long long>({c.sm_count / 2 / tiles, 4, p.k_stages}));
+    const int want = static_cast<int>(std::min<long long>({c.sm_count / 2 / tiles, sp24::kMaxDxSplits, p.k_stages}));
     p.splits = want > 1 ? dx_splits<DT>(tiles, want) : 1;
     st = p.splits > 1 ? launch_dx_split<DT>(c, a, b, p) : launch_ffn_pair<DT, sp24::kFfnDx>(c, a, b, p);
     if (st != SP24_OK) return st;

@@ -372,12 +372,20 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #pragma unroll
       for (int w = 0; w < C::G; ++w) {
         const uint32_t la = smem_u32(red + (w * BN + c) * C::RS + rl);
-        for (int src = 0; src < S; ++src) {
-          const float4 v = ld_dsmem_f4(mapa_shared(la, static_cast<uint32_t>(src)));
-          const uint32_t p[4] = {__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z),
-                                 __float_as_uint(v.w)};
+#pragma unroll 1
+        for (int s0 = 0; s0 < S; s0 += 4) {   // four loads on their way before the first sum
+          float4 v[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[w][j] = src == 0 ? p[j] : stream_add<OP>(acc[w][j], p[j]);
+          for (int i = 0; i < 4; ++i)
+            if (s0 + i < S) v[i] = ld_dsmem_f4(mapa_shared(la, static_cast<uint32_t>(s0 + i)));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (s0 + i >= S) break;
+            const uint32_t p[4] = {__float_as_uint(v[i].x), __float_as_uint(v[i].y), __float_as_uint(v[i].z),
+                                   __float_as_uint(v[i].w)};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[w][j] = s0 + i == 0 ? p[j] : stream_add<OP>(acc[w][j], p[j]);
+          }
         }
       }
       const long long t = nb * BN + c;
