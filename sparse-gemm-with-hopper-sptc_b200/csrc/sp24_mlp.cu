@@ -161,9 +161,9 @@ sp24_status check_scaled(const sp24_scaled_desc* d) {
 }
 
 // ------------------------------------------------------------------ gated feed-forward
-// fp32 row stride of the saved planes, 16-bit row stride of the dg / du planes:
-// rows start on 32- and 16-byte boundaries.
-inline int64_t ffn_ld(int f) { return static_cast<int64_t>(round_up(static_cast<size_t>(f), 8)); }
+// Row stride of the saved fp32 planes and of the 16-bit dg / du planes: whole
+// 128-byte lines, so that no row of a TMA box straddles two.
+inline int64_t ffn_ld(int f) { return static_cast<int64_t>(round_up(static_cast<size_t>(f), 64)); }
 
 sp24_status check_ffn(const sp24_ffn_desc* d) {
   if (d == nullptr) return SP24_ERR_ARG;

@@ -80,7 +80,7 @@ FFN = dict(dtype=1, t=4, h=64, f=96, act=1, x=P, w_gate=P, w_up=P)
     (dict(ldx=63), 1), (dict(ld_gate=56), 1), (dict(ld_up=8), 1),
     (dict(x=None), 8), (dict(w_gate=None), 8), (dict(w_up=None), 8),
     (dict(x=P + 2), 2), (dict(w_up=P + 8), 2), (dict(ldx=68), 2), (dict(h=63), 2),
-    (dict(saved=P, saved_bytes=4 * 2 * 96 * 4 - 1), 9),
+    (dict(saved=P, saved_bytes=4 * 2 * 128 * 4 - 1), 9),
     (dict(t=0, x=None), 0),
 ])
 def test_ffn_forward_refusals(kw, code):
@@ -116,8 +116,8 @@ def test_ffn_backward_refusals(kw, gkw, code):
 
 def test_ffn_buffer_sizes():
     lib = sp24.load()
-    assert lib.sp24_ffn_saved_bytes(3, 10) == 3 * 2 * 16 * 4     # rows of 16 floats
-    assert lib.sp24_ffn_workspace_bytes(3, 10) == 3 * 2 * 16 * 2
+    assert lib.sp24_ffn_saved_bytes(3, 10) == 3 * 2 * 64 * 4     # rows of 64 values
+    assert lib.sp24_ffn_workspace_bytes(3, 10) == 3 * 2 * 64 * 2
     assert lib.sp24_ffn_saved_bytes(0, 10) == lib.sp24_ffn_workspace_bytes(5, 0) == 0
     assert lib.sp24_ffn_saved_bytes(70000, 14336) == 70000 * 2 * 14336 * 4   # past 32 bits
 
