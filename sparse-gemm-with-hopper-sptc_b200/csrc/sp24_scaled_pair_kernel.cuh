@@ -20,13 +20,14 @@
 //                     buffers, for calls that do not fill the GPU with the other.
 // 14336 x 4096 int8, 4096 tokens (481 dense-equivalent GFLOP): 134 us in a burst,
 // 145 held under the 1000 W cap at 1.69 GHz, where the MMAs alone would take 86.
-// Shared memory bounds the main loop (per stage and SM the MMAs read 88 KB and
-// the copies write 68, 97 bytes a clock together): without its stores the
-// kernel takes 115 us, without its MMAs 114.  Measured and not kept: 128-byte
-// store lines (144 against 144), cache policies on weights or output (the same),
-// both accumulators packed before the first store (164), starting block 0 while
-// block 1 drains (148; with three stages ahead 147), 128-deep stages in a ring
-// twice as long (188: their 64-byte weight rows load slower).
+// Filling the stages and feeding the MMAs slow each other: without its stores the
+// kernel takes 115 us, without its MMAs 114, without its loads 117.  Measured and
+// not kept: 128-byte store lines (144 against 144), cache policies on weights or
+// output (the same), both accumulators packed before the first store (164),
+// starting block 0 while block 1 drains (148; with three stages ahead 147), three
+// accumulators of 160 columns, so that every epilogue overlaps (155 against 141),
+// one block x 224 tokens with two accumulators (146 against 144), 128-deep stages
+// in a ring twice as long (188: their 64-byte weight rows load slower).
 //
 // Accumulator lanes are weight rows, i.e. neighbouring features of a token's
 // output row: a warp's store of one token is one contiguous 64-byte run.
