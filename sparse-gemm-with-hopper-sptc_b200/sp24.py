@@ -390,11 +390,12 @@ _PACK_GRADS = struct.Struct("@QqQqQqQqQN").pack
 def _rows2d(t, what, cols=None, rows=None):
     """(t, row stride) of a matrix whose rows are contiguous, any row stride;
     others are copied.  A single row's stride says nothing: 0."""
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) != 2:
         raise ValueError(f"{what}: a 2-D tensor is wanted")
-    r, c = t.shape
+    r, c = shape
     if (cols is not None and c != cols) or (rows is not None and r != rows):
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected "
+        raise ValueError(f"{what}: shape {tuple(shape)}, expected "
                          f"({'any' if rows is None else rows}, {'any' if cols is None else cols})")
     ld, step = t.stride()
     if r > 1 and ld < c or c > 1 and step != 1:
@@ -407,9 +408,10 @@ def _tma_rows(t, what, cols=None, rows=None):
     """_rows2d whose rows also start on 16-byte boundaries (TMA operands):
     others are copied into padded rows first."""
     t, ld = _rows2d(t, what, cols, rows)
-    unit = 16 // t.element_size()
-    if t.data_ptr() % 16 == 0 and (ld or t.shape[1]) % unit == 0:
+    size = t.element_size()
+    if (t.data_ptr() | (ld or t.shape[1]) * size) & 15 == 0:
         return t, ld
+    unit = 16 // size
     ld = (t.shape[1] + unit - 1) // unit * unit
     padded = t.new_empty((t.shape[0], ld))[:, :t.shape[1]]
     padded.copy_(t)
@@ -417,13 +419,14 @@ def _tma_rows(t, what, cols=None, rows=None):
 
 
 def _same_device(first, *rest):
-    dev = first.device
-    if dev.type != "cuda":
-        raise ValueError(f"CUDA tensors are wanted, not {dev}")
+    """Index of the CUDA device that holds all of them."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError(f"CUDA tensors are wanted, not {first.device}")
     for t in rest:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on several devices: {dev}, {t.device}")
-    return dev.index
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"tensors on several devices: {first.device}, {t.device}")
+    return index
 
 
 def _on(index, stream, call, *args):
@@ -514,7 +517,8 @@ def _vector_f32(t, size, what):
         return None, 0
     if t.dtype != torch.float32 or t.numel() != size:
         raise ValueError(f"{what}: {size} float32 values are wanted")
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t, t.data_ptr()
 
 
