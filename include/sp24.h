@@ -330,7 +330,7 @@ sp24_status sp24_gemm_scaled(const sp24_scaled_desc* d, sp24_stream_t stream);
    the backward pass in fp32 through `saved`.  dg and du are rounded to dtype
    (they are tensor-core operands); every output is rounded once.
    x, w_gate and w_up rows must start on 16-byte boundaries (SP24_ERR_ALIGN);
-   so must the workspace, and saved on a 32-byte one.  out, d_out and the gradients have no alignment
+   saved and the workspace on 32-byte ones.  out, d_out and the gradients have no alignment
    rule. */
 typedef struct sp24_ffn_desc {
   sp24_dtype dtype;            /* SP24_F16 or SP24_BF16: every tensor below */
@@ -359,7 +359,7 @@ typedef struct sp24_ffn_grads {
   size_t workspace_bytes;
 } sp24_ffn_grads;
 size_t sp24_ffn_saved_bytes(int t, int f);
-size_t sp24_ffn_workspace_bytes(int t, int f);
+size_t sp24_ffn_workspace_bytes(int t, int h, int f);
 sp24_status sp24_ffn_forward(const sp24_ffn_desc* d, void* out, int64_t ld_out,
                              sp24_stream_t stream);
 sp24_status sp24_ffn_backward(const sp24_ffn_desc* d, const sp24_ffn_grads* g,

@@ -42,7 +42,9 @@ struct FfnParams {
   int k_stages;            // 64-deep stages of one tile
   int plane;               // dx: stages per plane; dw: row tiles per plane
   int group_m;
-  int splits;              // K-split form: pairs per cluster
+  int splits;              // dx: K slices a tile (K-split form: pairs per cluster)
+  float* partial;          // planes of m x ld_partial sums, a slice each, or null
+  long long ld_partial;
   void *out0, *out1;       // dw: dw_gate, dw_up; else out0
   long long ld_out0, ld_out1;
   int vec_out;             // 2: rows start on 32 bytes, 1: on 16, 0: neither
@@ -161,10 +163,13 @@ SP24_DEV void ffn_tile(const FfnParams& P, int t, int& mt, int& nt) {
 // tmA0 / tmA1, tmB0 / tmB1: the operands' two planes (forward: A is x, B0 and B1
 // are Wg and Wu; dx: A planes dg and du, B planes Wg and Wu; dw: A planes dg
 // and du, B is x).
-// KS = 0: clusters of 2, persistent over the tiles.  KS = 1 (few tiles): a
-// cluster of 2 S CTAs computes one tile, pair p its K slice p; each CTA parks its
-// fp32 partial tile in its idle ring, and the pairs' partials are summed in
-// order over distributed shared memory.
+// KS = 0: clusters of 2, persistent over the units of work.  These are the tiles,
+// or (dx over so few tiles that four pairs each would leave most idle) K slices
+// of them, whose fp32 sums go to a plane of the workspace each and are added up
+// by ffn_dx_sum_kernel.
+// KS = 1 (dx over few tiles): a cluster of 2 S CTAs computes one tile, pair p its
+// K slice p; each CTA parks its fp32 partial tile in its idle ring, and the
+// pairs' partials are summed in order over distributed shared memory.
 template <int DT, int MODE, int KS>
 SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, const CUtensorMap& tmB0,
                             const CUtensorMap& tmB1, const FfnParams& P) {
@@ -189,11 +194,15 @@ SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, co
   const bool leader = prank == 0;
   const uint16_t pair_mask = static_cast<uint16_t>(3u << lead);
   const int pair = KS ? static_cast<int>(blockIdx.x) / (2 * P.splits) : static_cast<int>(blockIdx.x >> 1);
-  const int num_tiles = P.m_tiles * P.n_tiles;
-  const int npairs = KS ? num_tiles : static_cast<int>(gridDim.x >> 1);   // KS: one tile
-  const int split = KS ? static_cast<int>(rank >> 1) : 0;
-  const int ks0 = KS ? P.k_stages * split / P.splits : 0;
-  const int ks1 = KS ? P.k_stages * (split + 1) / P.splits : P.k_stages;
+  const int slices = !KS && MODE == kFfnDx ? P.splits : 1;   // units a tile
+  const int num_units = P.m_tiles * P.n_tiles * slices;
+  const int npairs = KS ? num_units : static_cast<int>(gridDim.x >> 1);   // KS: one tile
+  // K stages [first, last) of unit t.
+  auto k_range = [&](int t, int& first, int& last) {
+    const int all = KS ? P.splits : slices, one = KS ? static_cast<int>(rank >> 1) : t % slices;
+    first = static_cast<int>(static_cast<long long>(P.k_stages) * one / all);
+    last = static_cast<int>(static_cast<long long>(P.k_stages) * (one + 1) / all);
+  };
   const uint64_t tmo = P.timeout_ns;
 
   if (threadIdx.x == 0) {
@@ -242,9 +251,10 @@ SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, co
     uint32_t ph = 0;
     bool ok = true;
     uint32_t used_mask = 0, used_ph = 0;   // slots of the leader's barrier with copies in flight
-    for (int t = pair; t < num_tiles && ok; t += npairs) {
-      int mt, nt;
-      ffn_tile(P, t, mt, nt);
+    for (int t = pair; t < num_units && ok; t += npairs) {
+      int mt, nt, ks0, ks1;
+      ffn_tile(P, t / slices, mt, nt);
+      k_range(t, ks0, ks1);
       const int mplane = MODE == kFfnDw && mt >= P.plane ? 1 : 0;
       if (MODE == kFfnDw) mt -= mplane * P.plane;
       // First row (or, MN-major, first column) of this CTA's 128.
@@ -288,7 +298,9 @@ SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, co
       int s = 0, buf = 0;
       uint32_t ph = 0, aph = 0;
       bool ok = true, any = false;
-      for (int t = pair; t < num_tiles && ok; t += npairs) {
+      for (int t = pair; t < num_units && ok; t += npairs) {
+        int ks0, ks1;
+        k_range(t, ks0, ks1);
         if (!mbar_wait_warp<true>(&acce_bar[buf], aph ^ 1u, &abort_sh, tmo)) {
           ok = false;
           break;
@@ -336,9 +348,9 @@ SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, co
     const uint32_t acce0 = mapa_shared(smem_u32(&acce_bar[0]), lead);
     int buf = 0;
     uint32_t aph = 0;
-    for (int t = pair; t < num_tiles; t += npairs) {
+    for (int t = pair; t < num_units; t += npairs) {
       int mt, nt;
-      ffn_tile(P, t, mt, nt);
+      ffn_tile(P, t / slices, mt, nt);
       const int mplane = MODE == kFfnDw && mt >= P.plane ? 1 : 0;
       if (MODE == kFfnDw) mt -= mplane * P.plane;
       bool ok = true;
@@ -370,6 +382,11 @@ SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, co
             *reinterpret_cast<uint4*>(red + j) = make_uint4(r0[j], r0[j + 1], r0[j + 2], r0[j + 3]);
             *reinterpret_cast<uint4*>(red + 32 + j) = make_uint4(r1[j], r1[j + 1], r1[j + 2], r1[j + 3]);
           }
+        } else if (MODE == kFfnDx && P.partial != nullptr) {
+          float* part = P.partial + (t % slices) * (P.m * P.ld_partial);
+          const int col0 = nt * 256 + half * 128 + c * 64;
+          store_run32_f32(part, P.ld_partial, r0, row0, P.m, col0, P.n);
+          store_run32_f32(part, P.ld_partial, r1, row0, P.m, col0 + 32, P.n);
         } else if constexpr (MODE == kFfnForward) {
           const int col0 = nt * 128 + half * 64;
 #pragma unroll
@@ -410,6 +427,7 @@ SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, co
     const int S = P.splits;
     int mt, nt;
     ffn_tile(P, pair, mt, nt);
+    const int split = static_cast<int>(rank >> 1);
     const int r0 = 128 * split / S, rows = 128 * (split + 1) / S - r0;
     const float* red = reinterpret_cast<const float*>(smem);
     for (int i = threadIdx.x; i < rows * 64; i += kPairThreads) {
@@ -460,6 +478,54 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                         const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
                         const FfnParams P) {
   ffn_pair_body<DT, kFfnDx, 1>(tmA0, tmA1, tmB0, tmB1, P);
+}
+
+// dx from the K slices' planes of m x ld fp32 sums: a block finishes 32 runs of
+// eight columns, its warp w adding up slices [w S / 8, (w + 1) S / 8) of each (the
+// slices are many where the runs are few, and one thread's chain of loads would
+// be all latency); the eight sums are then added in order.  VEC: dx's rows start
+// on 16 bytes.
+template <int DT, int VEC>
+__global__ void __launch_bounds__(256)
+    ffn_dx_sum_kernel(const float* __restrict__ part, int splits, int m, int n, long long ld, void* __restrict__ out,
+                      long long ldo) {
+  __shared__ float4 sums[8][2][32];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int per_row = (n + 7) / 8, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const long long unit = blockIdx.x * 32LL + lane, plane = m * ld;
+  const long long row = unit / per_row;
+  const int col = static_cast<int>(unit - row * per_row) * 8;
+  float4 a = make_float4(0, 0, 0, 0), b = a;
+  if (row < m) {
+    const float* p = part + row * ld + col;
+#pragma unroll 4
+    for (int s = splits * w / 8; s < splits * (w + 1) / 8; ++s) {
+      const float4 x = *reinterpret_cast<const float4*>(p + s * plane);
+      const float4 y = *reinterpret_cast<const float4*>(p + s * plane + 4);
+      a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+      b.x += y.x, b.y += y.y, b.z += y.z, b.w += y.w;
+    }
+  }
+  sums[w][0][lane] = a;
+  sums[w][1][lane] = b;
+  __syncthreads();
+  if (w != 0 || row >= m) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    const float4 x = sums[i][0][lane], y = sums[i][1][lane];
+    a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+    b.x += y.x, b.y += y.y, b.z += y.z, b.w += y.w;
+  }
+  const uint32_t k[4] = {pack16<DT>(a.x, a.y), pack16<DT>(a.z, a.w), pack16<DT>(b.x, b.y), pack16<DT>(b.z, b.w)};
+  uint16_t* o = static_cast<uint16_t*>(out) + row * ldo + col;
+  if (VEC && col + 8 <= n) {
+    *reinterpret_cast<uint4*>(o) = make_uint4(k[0], k[1], k[2], k[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (col + j < n) o[j] = static_cast<uint16_t>(k[j / 2] >> (16 * (j & 1)));
+  }
 }
 
 // dg = d_out u act'(g) and du = d_out act(g) from the saved fp32 sums, rounded

@@ -165,6 +165,18 @@ sp24_status check_scaled(const sp24_scaled_desc* d) {
 // 128-byte lines, so that no row of a TMA box straddles two.
 inline int64_t ffn_ld(int f) { return static_cast<int64_t>(round_up(static_cast<size_t>(f), 64)); }
 
+inline size_t dgu_bytes(int t, int f) { return static_cast<size_t>(t) * 2 * ffn_ld(f) * 2; }
+
+// K slices of a dx tile that go through the workspace: where the tiles are so few
+// that clusters of four pairs would leave most of the 74 idle, as many slices as
+// there are pairs for them, of at least eight stages each; else none.
+int dx_slices(int t, int h, int f) {
+  const long long tiles = ((t + 255LL) / 256) * ((h + 255LL) / 256);
+  const long long stages = 2 * ((f + 63LL) / 64);
+  const long long slices = std::min(74 / tiles, stages / 8);
+  return slices > sp24::kMaxDxSplits ? static_cast<int>(slices) : 0;
+}
+
 sp24_status check_ffn(const sp24_ffn_desc* d) {
   if (d == nullptr) return SP24_ERR_ARG;
   if (!is_16bit(d->dtype)) return SP24_ERR_ARG;
@@ -202,7 +214,7 @@ sp24_status launch_ffn_pair(const FfnCall& c, const CUtensorMap (&a)[2], const C
   if (st != SP24_OK) return st;
   p.status = c.status;
   p.timeout_ns = kDefaultTimeoutNs;
-  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles * std::max(1, p.splits);
   if (tiles > 0x7fffffff / 2) return SP24_ERR_SHAPE;
   const unsigned pairs = static_cast<unsigned>(std::min<long long>(tiles, c.sm_count / 2));
   return launch_gemm_kernel(kern, 2 * pairs, sp24::kPairThreads, C::SMEM_BYTES, c.stream, 0, true,
@@ -465,9 +477,9 @@ sp24_status launch_dx_split(const FfnCall& c, const CUtensorMap (&a)[2], const C
                             static_cast<unsigned>(2 * p.splits), true, a[0], a[1], b[0], b[1], p);
 }
 
-// Pairs per cluster of the K-split dx; 1 where the form does not apply.
+// Pairs per cluster of the K-split dx; 1 where no such clusters fit.
 template <int DT>
-int dx_splits(long long tiles, int want) {
+int dx_cluster(long long tiles, int want) {
   constexpr int smem = sp24::FfnCfg<DT, sp24::kFfnDx>::SMEM_BYTES;
   static std::atomic<bool> attr_set[kMaxDevices];
   auto kern = sp24::ffn_dx_split_kernel<DT>;
@@ -503,12 +515,27 @@ sp24_status ffn_backward(const FfnCall& c, const sp24_ffn_desc* d, const sp24_ff
     p.group_m = 8;
     p.out0 = g->dx, p.ld_out0 = stride_or(g->ld_dx, d->h), p.vec_out = out_vec(g->dx, p.ld_out0);
     // Few tiles: K split over the pairs of a cluster (777 x 1000, f = 2744, 16
-    // tiles of 86 stages: 48.3 -> 27.8 us with four, dg and du included).
+    // tiles of 86 stages: 45.0 -> 19.8 us with four; through the workspace 23.4).
+    // Very few: split further, through the workspace (40 x 112, f = 12344, one tile:
+    // 35.4 us with four pairs, 11.7 with 48 slices; 64 x 4096, f = 14336 keeps four).
     const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+    const int slices = dx_slices(d->t, d->h, d->f);
     const int want = static_cast<int>(std::min<long long>({c.sm_count / 2 / tiles, sp24::kMaxDxSplits, p.k_stages}));
-    p.splits = want > 1 ? dx_splits<DT>(tiles, want) : 1;
-    st = p.splits > 1 ? launch_dx_split<DT>(c, a, b, p) : launch_ffn_pair<DT, sp24::kFfnDx>(c, a, b, p);
+    p.splits = slices > 0 ? slices : want > 1 ? dx_cluster<DT>(tiles, want) : 1;
+    if (slices > 0) {
+      p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(g->workspace) + dgu_bytes(d->t, d->f));
+      p.ld_partial = ffn_ld(d->h);
+    }
+    st = slices == 0 && p.splits > 1 ? launch_dx_split<DT>(c, a, b, p) : launch_ffn_pair<DT, sp24::kFfnDx>(c, a, b, p);
     if (st != SP24_OK) return st;
+    if (slices > 0) {
+      const long long runs = static_cast<long long>(d->t) * ((d->h + 7) / 8);
+      auto sum = p.vec_out > 0 ? sp24::ffn_dx_sum_kernel<DT, 1> : sp24::ffn_dx_sum_kernel<DT, 0>;
+      st = launch_gemm_kernel(sum, static_cast<unsigned>((runs + 31) / 32), 256, 0, c.stream, 0, true,
+                              static_cast<const float*>(p.partial), p.splits, d->t, d->h, p.ld_partial, p.out0,
+                              p.ld_out0);
+      if (st != SP24_OK) return st;
+    }
   }
   if (g->dw_gate != nullptr) {
     st = encode_16(&a[0], dg, d->t, d->f, ldw, 64);
@@ -559,8 +586,10 @@ size_t sp24_ffn_saved_bytes(int t, int f) {
   return t <= 0 || f <= 0 ? 0 : static_cast<size_t>(t) * 2 * ffn_ld(f) * sizeof(float);
 }
 
-size_t sp24_ffn_workspace_bytes(int t, int f) {
-  return t <= 0 || f <= 0 ? 0 : static_cast<size_t>(t) * 2 * ffn_ld(f) * 2;
+size_t sp24_ffn_workspace_bytes(int t, int h, int f) {
+  if (t <= 0 || h <= 0 || f <= 0) return 0;
+  // planes of dg and du, then the slices' sums
+  return dgu_bytes(t, f) + static_cast<size_t>(dx_slices(t, h, f)) * t * ffn_ld(h) * sizeof(float);
 }
 
 sp24_status sp24_ffn_forward(const sp24_ffn_desc* d, void* out, int64_t ld_out,
@@ -592,9 +621,9 @@ sp24_status sp24_ffn_backward(const sp24_ffn_desc* d, const sp24_ffn_grads* g,
   if (d->t > 0) {
     if (g->d_out == nullptr || d->saved == nullptr) return SP24_ERR_ARG;
     if (d->saved_bytes < sp24_ffn_saved_bytes(d->t, d->f) || g->workspace == nullptr ||
-        g->workspace_bytes < sp24_ffn_workspace_bytes(d->t, d->f))
+        g->workspace_bytes < sp24_ffn_workspace_bytes(d->t, d->h, d->f))
       return SP24_ERR_WORKSPACE;
-    if (!aligned16(g->workspace)) return SP24_ERR_ALIGN;
+    if (!aligned32(g->workspace)) return SP24_ERR_ALIGN;
   }
   DeviceInfo* di = nullptr;
   st = device_info(&di);

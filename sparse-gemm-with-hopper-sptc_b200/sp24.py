@@ -197,8 +197,9 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.sp24_gemm_scaled.argtypes = [c_void_p, c_void_p]
     lib.sp24_ffn_forward.argtypes = [c_void_p, c_void_p, c_int64, c_void_p]
     lib.sp24_ffn_backward.argtypes = [c_void_p, c_void_p, c_void_p]
+    lib.sp24_ffn_saved_bytes.argtypes = [c_int, c_int]
+    lib.sp24_ffn_workspace_bytes.argtypes = [c_int, c_int, c_int]
     for name in ("sp24_ffn_saved_bytes", "sp24_ffn_workspace_bytes"):
-        getattr(lib, name).argtypes = [c_int, c_int]
         getattr(lib, name).restype = c_size_t
     for name in ("sp24_gemm_scaled", "sp24_ffn_forward", "sp24_ffn_backward",
                  "sp24_gemm", "sp24_gemm_noalloc", "sp24_gemm_fused", "sp24_gemm_allgather",
@@ -609,7 +610,7 @@ def _ffn_backward(s, d_out, x, w_gate, w_up, saved, act, need_dx, need_dw):
     dw_gate = dw_up = None
     if need_dw:
         dw_gate, dw_up = x.new_empty((f, h)), x.new_empty((f, h))
-    ws = x.new_empty((lib.sp24_ffn_workspace_bytes(t, f),), dtype=torch.uint8)
+    ws = x.new_empty((lib.sp24_ffn_workspace_bytes(t, h, f),), dtype=torch.uint8)
     d = _PACK_FFN(*args, saved.data_ptr(), saved.nbytes, 0)
     g = _PACK_GRADS(d_out.data_ptr(), ldd, _ptr(dx), 0, _ptr(dw_gate), 0, _ptr(dw_up), 0,
                     ws.data_ptr(), ws.nbytes)

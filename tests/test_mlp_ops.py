@@ -106,7 +106,7 @@ def test_ffn_forward_refusals(kw, code):
 ])
 def test_ffn_backward_refusals(kw, gkw, code):
     lib = sp24.load()
-    need = lib.sp24_ffn_workspace_bytes(4, 96)
+    need = lib.sp24_ffn_workspace_bytes(4, 64, 96)
     base = dict(FFN, saved=P, saved_bytes=lib.sp24_ffn_saved_bytes(4, 96))
     grads = dict(d_out=P, dx=P, dw_gate=P, dw_up=P, workspace=P, workspace_bytes=need)
     d = _fill(sp24.FfnDesc(), base, kw)
@@ -117,8 +117,10 @@ def test_ffn_backward_refusals(kw, gkw, code):
 def test_ffn_buffer_sizes():
     lib = sp24.load()
     assert lib.sp24_ffn_saved_bytes(3, 10) == 3 * 2 * 64 * 4     # rows of 64 values
-    assert lib.sp24_ffn_workspace_bytes(3, 10) == 3 * 2 * 64 * 2
-    assert lib.sp24_ffn_saved_bytes(0, 10) == lib.sp24_ffn_workspace_bytes(5, 0) == 0
+    assert lib.sp24_ffn_workspace_bytes(3, 8, 10) == 3 * 2 * 64 * 2   # one slice: dg and du alone
+    # 2 x 20 stages, slices of at least eight: five planes of 3 x 64 sums
+    assert lib.sp24_ffn_workspace_bytes(3, 8, 1280) == 3 * 2 * 1280 * 2 + 5 * 3 * 64 * 4
+    assert lib.sp24_ffn_saved_bytes(0, 10) == lib.sp24_ffn_workspace_bytes(5, 8, 0) == 0
     assert lib.sp24_ffn_saved_bytes(70000, 14336) == 70000 * 2 * 14336 * 4   # past 32 bits
 
 

@@ -415,7 +415,7 @@ def test_ffn_strides_padding_and_partial_gradients(t):
     assert lib.sp24_ffn_forward(ctypes.byref(d), o.data_ptr() + 2, f + 3, stream) == 0
     d.saved, d.saved_bytes = saved.data_ptr(), saved.numel()
     g = sp24.FfnGrads()
-    ws = torch.empty(lib.sp24_ffn_workspace_bytes(t, f), dtype=torch.uint8, device=DEV)
+    ws = torch.empty(lib.sp24_ffn_workspace_bytes(t, h, f), dtype=torch.uint8, device=DEV)
     bufs = [torch.full((r, h + 5), 9.0, device=DEV, dtype=dtype) for r in (t, f, f)]
     g.d_out, g.dx, g.dw_gate, g.dw_up = (v.data_ptr() for v in [dh] + bufs)
     g.ld_dx = g.ld_dgate = g.ld_dup = h + 5
