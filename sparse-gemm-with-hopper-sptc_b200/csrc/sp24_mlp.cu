@@ -283,7 +283,7 @@ sp24_status launch_stream_bn(const FfnCall& c, const CUtensorMap& a, const CUten
   // lets the next kernel's CTAs start their prologue beside this one's tail
   // (4096 x 4096, 1 token, back to back: 6.1 -> 5.6 us).
   p.ring = std::min(C::STAGES, (p.stages + p.splits - 1) / p.splits);
-  const int smem = std::max(p.ring * C::STAGE_BYTES, p.splits > 1 ? C::PARKED : 0) + 1024;
+  const int smem = std::max({p.ring * C::STAGE_BYTES + 1024, p.splits > 1 ? C::PARKED + 1024 : 0, C::MIN_SMEM});
   p.status = c.status;
   p.timeout_ns = kDefaultTimeoutNs;
   return launch_gemm_kernel(kern, static_cast<unsigned>(tiles * p.splits), sp24::kStreamThreads,

@@ -16,6 +16,14 @@
 // Accumulator lanes are weight rows, i.e. neighbouring features of a token's
 // output row: a warp's stores of one column are one contiguous run.
 //
+// Measured (device time in a graph, B200, weights from HBM at a copy rate of 6.5
+// TB/s): gated block 4096 -> 14336 bf16, one token: 235 MB in 39-41 us, 5.7-6.0 TB/s;
+// int8 product 4096 -> 14336, one token: 36.8 MB in 9.5 us, of which about 4 are
+// launch, first loads and drain (a 10 MB product takes 5.5); 32 tokens through
+// 14336 -> 4096 e4m3, K split in four: 11.5 us.  Bytes in flight decide the rest: a
+// ring of 110 KB instead of 190 costs 20%, and two CTAs an SM with half a ring
+// each 5-8%.
+//
 // Roles (6 warps): warp 0 loads (one copy a lane), warp 1 issues the MMAs,
 // warps 2-5 drain the accumulator.
 #pragma once
@@ -43,7 +51,6 @@ struct StreamParams {
   void* out;                // n x m
   long long ldo;
   int out_type;             // 0 f16, 1 bf16, 2 f32
-
   float* saved;             // ffn: planes of n x ld_saved, or null
   long long ld_saved;
   int silu;
@@ -81,6 +88,14 @@ struct StreamCfg {
                                         : COLS_NEEDED <= 128 ? 128
                                         : COLS_NEEDED <= 256 ? 256
                                                              : 512;
+  // The least shared memory a launch asks for.  CTAs that wait on one another
+  // (clusters) must never wait for TMEM that another waiting CTA holds, so no mix
+  // of this library's CTAs that fits an SM's shared memory may want more than its
+  // 512 columns: a CTA asks for at least the share of 228 KB that its columns are
+  // of 512, and for more than the pair kernels, which take all columns, leave free
+  // (50 KB).
+  static constexpr int MIN_SMEM = (TMEM_COLS * 228 / 512 < 56 ? 56 : static_cast<int>(TMEM_COLS * 228 / 512)) * 1024;
+  static_assert(MIN_SMEM <= SMEM_BYTES, "room for the least request");
   // Descriptor fields as in make_idesc_sparse; kind::i8 has D = s32 (2) and
   // signed A and B (1).
   static constexpr uint32_t IDESC =
