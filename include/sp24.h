@@ -271,8 +271,8 @@ sp24_status sp24_gemm_fused(const sp24_gemm_desc* d, const sp24_epilogue* e,
      sp24_quantize_rows  y = x                 (tokens, or the rows of a 16-bit
                          A_c: the weights of sp24_gemm_scaled, one scale per
                          output channel)
-   No alignment is required of any pointer or stride; rows whose pointers and
-   strides are 16-byte multiples take the vector path. */
+   No alignment is required of any pointer or stride; the wider the vectors that
+   divide the rows and start all of them aligned (16, 8 or 4 bytes), the faster. */
 typedef struct sp24_rowquant_desc {
   sp24_dtype dtype;            /* SP24_F16 or SP24_BF16: x, up, residual(_out), weight */
   sp24_dtype qdtype;           /* SP24_I8 or SP24_E4M3 */

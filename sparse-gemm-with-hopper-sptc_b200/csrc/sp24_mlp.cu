@@ -67,7 +67,7 @@ sp24_status launch_rows_kernel(const sp24::RowsParams& p, const DeviceInfo& di, 
   auto kern = sp24::rows_quant_kernel<DT, MODE, I8, V, VPT, ONE_WARP>;
   static std::atomic<bool> attr_set[kMaxDevices];
   static std::atomic<int> regs{0};
-  sp24_status st = ensure_kernel_attrs(kern, attr_set, V == 8 ? 2 * VPT * (ONE_WARP ? 256 : 1024) * 16 : 0);
+  sp24_status st = ensure_kernel_attrs(kern, attr_set, V > 1 ? 2 * VPT * (ONE_WARP ? 256 : 1024) * 2 * V : 0);
   if (st != SP24_OK) return st;
   if (regs.load(std::memory_order_relaxed) == 0) {
     cudaFuncAttributes a{};
@@ -75,10 +75,10 @@ sp24_status launch_rows_kernel(const sp24::RowsParams& p, const DeviceInfo& di, 
     regs.store((a.numRegs + 7) / 8 * 8, std::memory_order_relaxed);
   }
   const int inputs = p.up != nullptr || p.residual != nullptr ? 2 : 1;
-  const int smem = V == 8 ? inputs * VPT * static_cast<int>(threads) * 16 : 0;
+  const int smem = V > 1 ? inputs * VPT * static_cast<int>(threads) * 2 * V : 0;
   const int t = static_cast<int>(threads);
   int blocks = std::min({2048 / t, 65536 / (regs.load(std::memory_order_relaxed) * t), 32});
-  if (V == 8) blocks = std::min(blocks, kSmem / std::max(smem, 1));
+  if (V > 1) blocks = std::min(blocks, kSmem / std::max(smem, 1));
   blocks = std::max(blocks, 1);
   const long long per_block = ONE_WARP ? t / 32 : 1;
   const long long want = (p.rows + per_block - 1) / per_block;
@@ -100,8 +100,9 @@ sp24_status launch_rows_vpt(const sp24::RowsParams& p, const DeviceInfo& di, int
 // and more to gain from few warps a row: four (8192 x 4096 plain: 18.5 us; 20.6
 // with two, 22.7 with one), unless a warp covers the row with one (8192 x 256:
 // 4.4 us; 6.0 with four) or there are few rows, whose loads then go out at once.
-// Single elements (V = 1) want eight: fewer threads, more loads each (4096 x 1001
-// swiglu: 10.3 us; 12.0 with four).
+// Vectors of four and two values: four where they reach (norm 8192 x 4092 / 4094:
+// 43.9 / 62.5 us; 64.4 / 80.2 with eight), single elements eight (4096 x 1001
+// swiglu: 10.3 us; 12.0 with four, 12.7 with sixteen).
 template <int DT, int MODE, int I8, int V>
 sp24_status launch_rows_v(const sp24::RowsParams& p, const DeviceInfo& di, cudaStream_t s) {
   const int vecs = (p.cols + V - 1) / V;
@@ -112,7 +113,8 @@ sp24_status launch_rows_v(const sp24::RowsParams& p, const DeviceInfo& di, cudaS
     if ((norm || few) && vecs <= 2 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 2>(p, di, vecs, s);
     if (vecs <= 4 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 4>(p, di, vecs, s);
   } else {
-    if (vecs <= 8 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 8>(p, di, vecs, s);
+    if (V > 1 && vecs <= 4 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 4>(p, di, vecs, s);
+    if (V < 4 && vecs <= 8 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 8>(p, di, vecs, s);
   }
   return launch_gemm_kernel(sp24::rows_quant_long_kernel<DT, MODE, I8>,
                             static_cast<unsigned>(p.rows), 1024, 0, s, 0, true, p);
@@ -120,11 +122,19 @@ sp24_status launch_rows_v(const sp24::RowsParams& p, const DeviceInfo& di, cudaS
 
 template <int DT, int MODE, int I8>
 sp24_status launch_rows(const sp24::RowsParams& p, const DeviceInfo& di, cudaStream_t s) {
-  auto vec = [](const void* q, long long ld) { return q == nullptr || (aligned16(q) && ld % 8 == 0); };
-  const bool v8 = p.cols % 8 == 0 && vec(p.x, p.ldx) && vec(p.up, p.ld_up) &&
-                  vec(p.residual, p.ld_residual) && vec(p.residual_out, p.ld_residual_out) &&
-                  vec(p.weight, 0) && reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && p.ldq % 8 == 0;
-  return v8 ? launch_rows_v<DT, MODE, I8, 8>(p, di, s) : launch_rows_v<DT, MODE, I8, 1>(p, di, s);
+  // The widest vector that divides the rows and starts all of them aligned.
+  auto fits = [&](int v) {
+    auto in = [v](const void* q, long long ld) {
+      return q == nullptr || (reinterpret_cast<uintptr_t>(q) % (2 * v) == 0 && ld % v == 0);
+    };
+    return p.cols % v == 0 && in(p.x, p.ldx) && in(p.up, p.ld_up) && in(p.residual, p.ld_residual) &&
+           in(p.residual_out, p.ld_residual_out) && in(p.weight, 0) &&
+           reinterpret_cast<uintptr_t>(p.q) % v == 0 && p.ldq % v == 0;
+  };
+  return fits(8)   ? launch_rows_v<DT, MODE, I8, 8>(p, di, s)
+         : fits(4) ? launch_rows_v<DT, MODE, I8, 4>(p, di, s)
+         : fits(2) ? launch_rows_v<DT, MODE, I8, 2>(p, di, s)
+                   : launch_rows_v<DT, MODE, I8, 1>(p, di, s);
 }
 
 template <int MODE>

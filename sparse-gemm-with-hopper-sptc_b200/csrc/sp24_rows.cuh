@@ -75,14 +75,39 @@ SP24_DEV uint32_t codes2(float a, float b) {
   }
 }
 
-// V neighbouring values of a row as they lie in memory: 16 bytes (V = 8) or one
-// element.
+// V neighbouring values of a row as they lie in memory: one load of 2 V bytes, in
+// the low words of the result.
 template <int V>
 SP24_DEV uint4 load_raw(const void* p, long long i) {
   const uint16_t* q = static_cast<const uint16_t*>(p) + i;
-  if constexpr (V == 8) return *reinterpret_cast<const uint4*>(q);
-  else return make_uint4(*q, 0, 0, 0);
+  if constexpr (V == 8) {
+    return *reinterpret_cast<const uint4*>(q);
+  } else if constexpr (V == 4) {
+    const uint2 w = *reinterpret_cast<const uint2*>(q);
+    return make_uint4(w.x, w.y, 0, 0);
+  } else if constexpr (V == 2) {
+    return make_uint4(*reinterpret_cast<const uint32_t*>(q), 0, 0, 0);
+  } else {
+    return make_uint4(*q, 0, 0, 0);
+  }
 }
+// ... and V codes, two to a half word, or V 16-bit values, two to a word, back.
+template <int V>
+SP24_DEV void store_codes(uint8_t* q, const uint32_t (&k)[4]) {
+  if constexpr (V == 8) __stcs(reinterpret_cast<uint2*>(q), make_uint2(k[0] | k[1] << 16, k[2] | k[3] << 16));
+  else if constexpr (V == 4) __stcs(reinterpret_cast<uint32_t*>(q), k[0] | k[1] << 16);
+  else if constexpr (V == 2) *reinterpret_cast<uint16_t*>(q) = static_cast<uint16_t>(k[0]);
+  else *q = static_cast<uint8_t>(k[0]);
+}
+template <int V>
+SP24_DEV void store_raw(void* p, long long i, const uint32_t (&w)[4]) {
+  uint16_t* q = static_cast<uint16_t*>(p) + i;
+  if constexpr (V == 8) __stcs(reinterpret_cast<uint4*>(q), make_uint4(w[0], w[1], w[2], w[3]));
+  else if constexpr (V == 4) __stcs(reinterpret_cast<uint2*>(q), make_uint2(w[0], w[1]));
+  else if constexpr (V == 2) *reinterpret_cast<uint32_t*>(q) = w[0];
+  else *q = static_cast<uint16_t>(w[0]);
+}
+
 // The two values of one 32-bit word (V = 1: the one value and a zero).
 template <int DT>
 SP24_DEV float2 unpack2(uint32_t w) {
@@ -151,8 +176,13 @@ SP24_DEV float max_abs(float a, float b) {
   return r;
 }
 
-SP24_DEV void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+// Asynchronous copy of V 16-bit values (V = 8, 4, 2).
+template <int V>
+SP24_DEV void cp_async(void* dst, const void* src) {
+  if constexpr (V == 8)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(2 * V) : "memory");
 }
 SP24_DEV void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -186,16 +216,16 @@ SP24_DEV RowScale row_scale(uint32_t top, float gain) {
 // row costs one barrier (8192 x 4096: 39.6 us with one after the other).
 // ONE_WARP: a warp per row, blockDim.x / 32 rows a block; else a block per row.
 //
-// The grid is resident and walks the rows.  With V = 8 every thread has a slot
+// The grid is resident and walks the rows.  With V > 1 every thread has a slot
 // in shared memory for each of its vectors: it issues the copies of its next
 // row (cp.async) as soon as it has unpacked the current one, so loads stay in
 // flight through the reductions and stores.  A slot has one owner: no barrier
 // guards it, only the owner's own wait.
 template <int DT, int MODE, int I8, int V, int VPT, bool ONE_WARP>
 __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_quant_kernel(const RowsParams P) {
-  extern __shared__ uint4 slots[];   // V = 8: [input][VPT][blockDim.x]
+  extern __shared__ __align__(16) uint8_t slots[];   // V > 1: [input][VPT][blockDim.x] vectors
   __shared__ uint2 sh[2][32];
-  constexpr int H = V == 8 ? 4 : 1;  // pairs of values a vector
+  constexpr int H = V > 1 ? V / 2 : 1;   // words of two values a vector
   griddep_launch_dependents();
   const int tid = ONE_WARP ? threadIdx.x & 31 : threadIdx.x;
   const int step = ONE_WARP ? 32 : blockDim.x;
@@ -205,7 +235,8 @@ __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_quant_kernel(const
   const void* other = MODE == kRowsSwiglu ? P.up : P.residual;
   const long long ld_other = MODE == kRowsSwiglu ? P.ld_up : P.ld_residual;
   const bool two = MODE == kRowsSwiglu || (MODE == kRowsNorm && other != nullptr);
-  uint4* mine = slots + threadIdx.x;
+  // Slot of vector i of input w.
+  auto slot = [&](int w, int i) { return slots + ((w * VPT + i) * blockDim.x + threadIdx.x) * (2 * V); };
   auto fetch = [&](long long row) {
     const uint16_t* px = static_cast<const uint16_t*>(P.x) + row * P.ldx;
     const uint16_t* po = static_cast<const uint16_t*>(other) + row * ld_other;
@@ -213,14 +244,14 @@ __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_quant_kernel(const
     for (int i = 0; i < VPT; ++i) {
       const int c = (tid + i * step) * V;
       if (c < P.cols) {
-        cp_async16(mine + i * blockDim.x, px + c);
-        if (two) cp_async16(mine + (VPT + i) * blockDim.x, po + c);
+        cp_async<V>(slot(0, i), px + c);
+        if (two) cp_async<V>(slot(1, i), po + c);
       }
     }
   };
   if (r >= P.rows) return;
   griddep_wait();
-  if constexpr (V == 8) fetch(r);
+  if constexpr (V > 1) fetch(r);
   uint4 rw[VPT];   // past the row's end 0
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -233,14 +264,14 @@ __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_quant_kernel(const
     float2 v[VPT][H];
     float2 ss = make_float2(0.0f, 0.0f);
     float top = 0.0f;
-    if constexpr (V == 8) cp_async_wait_all();
+    if constexpr (V > 1) cp_async_wait_all();
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = (tid + i * step) * V;
       uint4 rx = make_uint4(0, 0, 0, 0), ro = rx;
       if (c < P.cols) {
-        rx = V == 8 ? mine[i * blockDim.x] : load_raw<V>(P.x, r * P.ldx + c);
-        if (two) ro = V == 8 ? mine[(VPT + i) * blockDim.x] : load_raw<V>(other, r * ld_other + c);
+        rx = V > 1 ? load_raw<V>(slot(0, i), 0) : load_raw<V>(P.x, r * P.ldx + c);
+        if (two) ro = V > 1 ? load_raw<V>(slot(1, i), 0) : load_raw<V>(other, r * ld_other + c);
       }
       const uint32_t wx[4] = {rx.x, rx.y, rx.z, rx.w}, wo[4] = {ro.x, ro.y, ro.z, ro.w};
       const uint32_t ww[4] = {rw[i].x, rw[i].y, rw[i].z, rw[i].w};
@@ -255,14 +286,10 @@ __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_quant_kernel(const
         v[i][j] = a;
       }
       if (MODE == kRowsNorm && P.residual_out != nullptr && c < P.cols) {
-        const long long o = r * P.ld_residual_out + c;
-        if constexpr (V == 8) {
-          __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(P.residual_out) + o),
-                 make_uint4(pack16<DT>(v[i][0].x, v[i][0].y), pack16<DT>(v[i][1].x, v[i][1].y),
-                            pack16<DT>(v[i][2].x, v[i][2].y), pack16<DT>(v[i][3].x, v[i][3].y)));
-        } else {
-          store16<DT>(P.residual_out, o, v[i][0].x);
-        }
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < H; ++j) w[j] = pack16<DT>(v[i][j].x, v[i][j].y);
+        store_raw<V>(P.residual_out, r * P.ld_residual_out + c, w);
       }
 #pragma unroll
       for (int j = 0; j < H; ++j) {
@@ -270,7 +297,7 @@ __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_quant_kernel(const
         top = max_abs(max_abs(top, v[i][j].x), v[i][j].y);
       }
     }
-    if constexpr (V == 8)
+    if constexpr (V > 1)
       if (r + stride < P.rows) fetch(r + stride);
     const RowStats st = row_reduce<ONE_WARP, MODE == kRowsNorm>(ss.x + ss.y, __float_as_uint(top), sh[parity]);
     parity ^= 1;
@@ -296,10 +323,7 @@ __global__ void __launch_bounds__(ONE_WARP ? 256 : 1024) rows_quant_kernel(const
         const float2 a = mul2(v[i][j], inv);
         k[j] = codes2<I8>(a.x, a.y);
       }
-      if constexpr (V == 8)
-        __stcs(reinterpret_cast<uint2*>(q + c), make_uint2(k[0] | k[1] << 16, k[2] | k[3] << 16));
-      else
-        q[c] = static_cast<uint8_t>(k[0]);
+      store_codes<V>(q + c, k);
     }
   }
 }

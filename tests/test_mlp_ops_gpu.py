@@ -74,7 +74,8 @@ def rmsnorm64(x, w, r, eps):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 4096), (3, 7), (5, 64), (2, 129), (17, 1000),
                                        (33, 2048), (4, 5000), (2, 8192), (3, 14336), (1, 16392),
-                                       (2, 40001)])
+                                       (2, 40001), (9, 4092), (300, 300), (7, 8190), (3, 10006),
+                                       (2, 16380), (2, 16386), (2, 8194)])
 def test_rows_sizes(rows, cols, dtype, qdtype):
     x, r = randn(rows, cols, seed=1, dtype=dtype), randn(rows, cols, seed=2, std=3.0, dtype=dtype)
     w = (1 + randn(cols, seed=3, std=0.1)).to(dtype)
@@ -93,7 +94,8 @@ def test_rows_sizes(rows, cols, dtype, qdtype):
 
 
 @pytest.mark.parametrize("cols,ld,off", [(64, 72, 0), (64, 65, 0), (64, 64, 1), (1000, 1016, 8),
-                                         (4096, 8192, 4096), (4097, 4100, 3)])
+                                         (4096, 8192, 4096), (4097, 4100, 3),
+                                         (100, 102, 2), (100, 104, 4), (96, 100, 4), (98, 98, 2), (64, 66, 0)])
 def test_rows_strides(cols, ld, off):
     """Any row stride and any start, including 2-byte aligned ones."""
     buf = [randn(9 * ld + off, seed=i, dtype=torch.bfloat16) for i in range(2)]
