@@ -3,10 +3,11 @@
 // product, or as they are.
 //
 // Bound by HBM: each input is read once and each output written once.  B200,
-// measured copy rate 6.5 TB/s: norm with residual 8192 x 4096 bf16 (235 MB) 39.0 us,
-// 6.0 TB/s; SwiGLU 4096 x 14336 (294 MB) 49.3 us, 6.0 TB/s; plain 8192 x 14336 (352 MB)
-// 55.7 us, 6.3 TB/s.  The SwiGLU is nearest to another limit: its exponential and
-// reciprocal keep their unit busy half of the time.
+// measured copy rate 6.5 TB/s, device time over rotating buffers: norm with residual
+// 8192 x 4096 bf16 (235 MB) 36.6 us, 6.4 TB/s; SwiGLU 4096 x 14336 (294 MB) 47.9 us,
+// 6.1 TB/s; plain 8192 x 14336 (352 MB) 55.7 us, 6.3 TB/s.  The SwiGLU is nearest to
+// another limit: its exponential and reciprocal keep their unit busy half of the
+// time.
 #pragma once
 
 #include <cuda_bf16.h>
