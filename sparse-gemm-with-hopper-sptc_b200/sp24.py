@@ -433,11 +433,16 @@ def _same_device(first, *rest):
 def _on(index, stream, call, *args):
     """call(raw stream, *args) with the tensors' device current and `stream`
     (None: the current one) torch's current stream, so that copies and outputs
-    made on the way are ordered with the kernels."""
+    made on the way are ordered with the kernels.  Inputs used on a stream that
+    was named are recorded with it: their memory outlives the call there."""
     import torch
     if stream is None and torch._C._cuda_getDevice() == index:
         return call(torch._C._cuda_getCurrentRawStream(index), *args)
     with torch.cuda.device(index), torch.cuda.stream(stream):
+        if stream is not None:
+            for t in args:
+                if isinstance(t, torch.Tensor):
+                    t.record_stream(stream)
         return call(torch._C._cuda_getCurrentRawStream(index), *args)
 
 

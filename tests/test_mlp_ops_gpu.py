@@ -607,3 +607,45 @@ def test_calls_from_several_threads():
     for t in threads:
         t.join()
     assert all(torch.equal(a, b) for p, q in zip(got, want) for a, b in zip(p, q))
+
+
+def test_products_past_32_bit_offsets():
+    """Outputs of more than 2^31 elements: the last rows, and the rows around the
+    element 2^31."""
+    n, wide, k = 150001, 14400, 64
+    at = torch.tensor([0, 2 ** 31 // wide - 1, 2 ** 31 // wide, 2 ** 31 // wide + 1, n - 2, n - 1], device=DEV)
+    a_c, image, w = weights_2of4(wide, k, sp24.I8, seed=1)
+    x = tokens_8bit(n, k, sp24.I8, seed=2)
+    sw, sx = torch.rand(wide, device=DEV) * 1e-3, torch.rand(n, device=DEV)
+    c = sp24.gemm_scaled(a_c, image, x, sw, sx)
+    check_scaled(c[at], x[at], w, sw, sx[at], None, sp24.I8, k)
+    del c
+    xb = randn(n, k, seed=3, dtype=torch.bfloat16)
+    wg, wu = (randn(wide, k, seed=s, std=0.09, dtype=torch.bfloat16) for s in (4, 5))
+    h, saved = sp24.ffn_gated(xb, wg, wu, save=True)
+    dh = torch.zeros_like(h)
+    dh[at] = randn(len(at), wide, seed=6, dtype=torch.bfloat16)
+    dx, dwg, dwu = sp24.ffn_gated_backward(dh, xb, wg, wu, saved)
+    # only the chosen tokens carry a gradient, so these are the whole sums
+    check_ffn(xb[at], wg, wu, dh[at], sp24.ACT_SILU, h[at], (dx[at], None, None))
+    few = sp24.ffn_gated(xb[at], wg, wu, save=True)[1]
+    _, eg, eu = sp24.ffn_gated_backward(dh[at].contiguous(), xb[at], wg, wu, few, need_dx=False)
+    assert torch.allclose(dwg.float(), eg.float(), rtol=2 ** -7, atol=1e-6)
+    assert torch.allclose(dwu.float(), eu.float(), rtol=2 ** -7, atol=1e-6)
+
+
+def test_inputs_freed_right_after_a_call_on_another_stream():
+    """A named stream's inputs may be freed at once: their memory is not handed
+    out again before the kernel has read it."""
+    side = torch.cuda.Stream()
+    want = sp24.quantize_rows(randn(4096, 4096, seed=1, dtype=torch.bfloat16))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        x = randn(4096, 4096, seed=1, dtype=torch.bfloat16)
+        side.wait_stream(torch.cuda.current_stream())
+        big = [sp24.quantize_rows(x, stream=side) for _ in range(4)]
+        del x
+        junk = torch.full((4096, 4096), 3.0, device=DEV, dtype=torch.bfloat16)
+        side.synchronize()
+        assert all(torch.equal(q, want[0]) and torch.equal(s, want[1]) for q, s in big)
+        del junk
