@@ -42,7 +42,7 @@
 namespace sp24 {
 
 enum : int { kFfnForward = 0, kFfnDx = 1, kFfnDw = 2 };
-constexpr int kMaxDxSplits = 4;   // pairs per cluster of the K-split dx: 8 CTAs
+constexpr int kFfnMaxSplits = 4;   // pairs per cluster of the K-split forms: 8 CTAs
 
 struct FfnParams {
   int m, n;                // rows of a plane's output, output columns (forward: f)
@@ -50,7 +50,7 @@ struct FfnParams {
   int k_stages;            // 64-deep stages of one tile
   int plane;               // dx: stages per plane; dw: row tiles per plane
   int group_m;
-  int splits;              // dx: K slices a tile (K-split form: pairs per cluster)
+  int splits;              // K-split forms: pairs per cluster; dx: else K slices a tile
   float* partial;          // planes of m x ld_partial sums, a slice each, or null
   long long ld_partial;
   void *out0, *out1;       // dw: dw_gate, dw_up; else out0
@@ -175,7 +175,7 @@ SP24_DEV void ffn_tile(const FfnParams& P, int t, int& mt, int& nt) {
 // or (dx over so few tiles that four pairs each would leave most idle) K slices
 // of them, whose fp32 sums go to a plane of the workspace each and are added up
 // by ffn_dx_sum_kernel.
-// KS = 1 (dx over few tiles): a cluster of 2 S CTAs computes one tile, pair p its
+// KS = 1 (forward or dx over few tiles): a cluster of 2 S CTAs computes one tile, pair p its
 // K slice p; each CTA parks its fp32 partial tile in its idle ring, and the
 // pairs' partials are summed in order over distributed shared memory.
 template <int DT, int MODE, int KS>
@@ -384,11 +384,13 @@ SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, co
           if (lane == 0) mbar_arrive_cluster(acce0 + buf * sizeof(uint64_t));
         }
         if constexpr (KS) {
-          float* red = reinterpret_cast<float*>(smem) + (q * 32 + lane) * C::RS + half * 128 + c * 64;
+          // Parked at the accumulator's own columns.
+          constexpr int R1 = MODE == kFfnForward ? 128 : 32;
+          float* red = reinterpret_cast<float*>(smem) + (q * 32 + lane) * C::RS + (c0 - tb);
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             *reinterpret_cast<uint4*>(red + j) = make_uint4(r0[j], r0[j + 1], r0[j + 2], r0[j + 3]);
-            *reinterpret_cast<uint4*>(red + 32 + j) = make_uint4(r1[j], r1[j + 1], r1[j + 2], r1[j + 3]);
+            *reinterpret_cast<uint4*>(red + R1 + j) = make_uint4(r1[j], r1[j + 1], r1[j + 2], r1[j + 3]);
           }
         } else if (MODE == kFfnDx && P.partial != nullptr) {
           float* part = P.partial + (t % slices) * (P.m * P.ld_partial);
@@ -430,26 +432,42 @@ SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, co
   cluster_sync();   // KS: every pair's partial is parked and visible (release / acquire)
   if constexpr (KS) {
     // CTA (slice p, half h) finishes rows [128 p / S, 128 (p + 1) / S) of its half
-    // of the tile, four columns a thread.
-    static_assert(MODE == kFfnDx, "the K-split form serves dx");
+    // of the tile, four output columns a thread.
+    static_assert(MODE != kFfnDw, "the K-split forms");
     const int S = P.splits;
     int mt, nt;
     ffn_tile(P, pair, mt, nt);
     const int split = static_cast<int>(rank >> 1);
     const int r0 = 128 * split / S, rows = 128 * (split + 1) / S - r0;
     const float* red = reinterpret_cast<const float*>(smem);
-    for (int i = threadIdx.x; i < rows * 64; i += kPairThreads) {
-      const int rl = r0 + (i >> 6), cl = (i & 63) * 4;
+    // Sum over the slices of four parked columns; all loads on their way first.
+    auto total = [&](int rl, int cl) {
       const uint32_t la = smem_u32(red + rl * C::RS + cl);
-      float4 v[kMaxDxSplits];   // all loads on their way before the first sum
+      float4 v[kFfnMaxSplits];
 #pragma unroll
-      for (int sp = 0; sp < kMaxDxSplits; ++sp)
+      for (int sp = 0; sp < kFfnMaxSplits; ++sp)
         if (sp < S) v[sp] = ld_dsmem_f4(mapa_shared(la, static_cast<uint32_t>(2 * sp + prank)));
       float4 a = v[0];
 #pragma unroll
-      for (int sp = 1; sp < kMaxDxSplits; ++sp)
+      for (int sp = 1; sp < kFfnMaxSplits; ++sp)
         if (sp < S) a.x += v[sp].x, a.y += v[sp].y, a.z += v[sp].z, a.w += v[sp].w;
-      const int row = mt * 256 + prank * 128 + rl, col = nt * 256 + cl;
+      return a;
+    };
+    constexpr int COLS = MODE == kFfnForward ? 128 : 256;   // output columns of a tile
+    for (int i = threadIdx.x; i < rows * (COLS / 4); i += kPairThreads) {
+      const int rl = r0 + i / (COLS / 4), cl = i % (COLS / 4) * 4;
+      float4 a = total(rl, cl);
+      const int row = mt * 256 + prank * 128 + rl, col = nt * COLS + cl;
+      if constexpr (MODE == kFfnForward) {
+        const float4 u = total(rl, 128 + cl);
+        if (P.saved != nullptr && row < P.m && col < P.n) {   // whole units, the last over the padding
+          float* g = P.saved + row * P.ld_saved + col;
+          *reinterpret_cast<float4*>(g) = a;
+          *reinterpret_cast<float4*>(g + P.m * P.ld_saved) = u;
+        }
+        a = make_float4(gate_act(a.x, P.silu) * u.x, gate_act(a.y, P.silu) * u.y, gate_act(a.z, P.silu) * u.z,
+                        gate_act(a.w, P.silu) * u.w);
+      }
       if (row >= P.m) continue;
       uint16_t* dst = static_cast<uint16_t*>(P.out0) + row * P.ld_out0 + col;
       const uint32_t w[2] = {pack16<DT>(a.x, a.y), pack16<DT>(a.z, a.w)};
@@ -480,12 +498,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 }
 
 // Launched with a run-time cluster of 2 * P.splits CTAs.
-template <int DT>
+template <int DT, int MODE>
 __global__ void __launch_bounds__(kPairThreads, 1)
-    ffn_dx_split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
+    ffn_split_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
                         const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
                         const FfnParams P) {
-  ffn_pair_body<DT, kFfnDx, 1>(tmA0, tmA1, tmB0, tmB1, P);
+  ffn_pair_body<DT, MODE, 1>(tmA0, tmA1, tmB0, tmB1, P);
 }
 
 // dx from the K slices' planes of m x ld fp32 sums: a block finishes 32 runs of

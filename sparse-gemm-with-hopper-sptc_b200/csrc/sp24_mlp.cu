@@ -184,7 +184,7 @@ int dx_slices(int t, int h, int f) {
   const long long tiles = ((t + 255LL) / 256) * ((h + 255LL) / 256);
   const long long stages = 2 * ((f + 63LL) / 64);
   const long long slices = std::min(74 / tiles, stages / 8);
-  return slices > sp24::kMaxDxSplits ? static_cast<int>(slices) : 0;
+  return slices > sp24::kFfnMaxSplits ? static_cast<int>(slices) : 0;
 }
 
 sp24_status check_ffn(const sp24_ffn_desc* d) {
@@ -456,6 +456,28 @@ sp24_status ffn_forward_few(const FfnCall& c, const sp24_ffn_desc* d, void* out,
   return launch_stream<DT == 0 ? sp24::kStreamF16 : sp24::kStreamBF16>(c, a, a2, b, p);
 }
 
+// Few tiles of the forward pass or of dx, K split over the pairs of a cluster;
+// p.splits = 1 where that does not apply (no two pairs a tile, no such clusters).
+template <int DT, int MODE>
+sp24_status launch_ffn_split(const FfnCall& c, const CUtensorMap (&a)[2], const CUtensorMap (&b)[2],
+                             sp24::FfnParams p, int want) {
+  using C = sp24::FfnCfg<DT, MODE>;
+  constexpr auto kern = sp24::ffn_split_kernel<DT, MODE>;
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  p.splits = 1;
+  if (want > 1) {
+    static std::atomic<bool> attr_set[kMaxDevices];
+    const sp24_status st = ensure_kernel_attrs(kern, attr_set, C::SMEM_BYTES);
+    if (st != SP24_OK) return st;
+    p.splits = resident_splits<kern>(sp24::kPairThreads, C::SMEM_BYTES, tiles, 2, want);
+  }
+  if (p.splits <= 1) return launch_ffn_pair<DT, MODE>(c, a, b, p);
+  p.status = c.status;
+  p.timeout_ns = kDefaultTimeoutNs;
+  return launch_gemm_kernel(kern, static_cast<unsigned>(tiles * 2 * p.splits), sp24::kPairThreads, C::SMEM_BYTES,
+                            c.stream, static_cast<unsigned>(2 * p.splits), true, a[0], a[1], b[0], b[1], p);
+}
+
 template <int DT>
 sp24_status ffn_forward(const FfnCall& c, const sp24_ffn_desc* d, void* out, int64_t ld_out) {
   if (d->t <= kStreamMaxTokens) return ffn_forward_few<DT>(c, d, out, ld_out);
@@ -473,28 +495,13 @@ sp24_status ffn_forward(const FfnCall& c, const sp24_ffn_desc* d, void* out, int
   p.out0 = out, p.ld_out0 = ld_out, p.vec_out = out_vec(out, ld_out);
   p.saved = static_cast<float*>(d->saved), p.ld_saved = ffn_ld(d->f);
   p.silu = d->act == SP24_ACT_SILU;
-  return launch_ffn_pair<DT, sp24::kFfnForward>(c, a, b, p);
-}
-
-template <int DT>
-sp24_status launch_dx_split(const FfnCall& c, const CUtensorMap (&a)[2], const CUtensorMap (&b)[2],
-                            sp24::FfnParams p) {
-  p.status = c.status;
-  p.timeout_ns = kDefaultTimeoutNs;
-  return launch_gemm_kernel(sp24::ffn_dx_split_kernel<DT>,
-                            static_cast<unsigned>(p.m_tiles * p.n_tiles * 2 * p.splits), sp24::kPairThreads,
-                            sp24::FfnCfg<DT, sp24::kFfnDx>::SMEM_BYTES, c.stream,
-                            static_cast<unsigned>(2 * p.splits), true, a[0], a[1], b[0], b[1], p);
-}
-
-// Pairs per cluster of the K-split dx; 1 where no such clusters fit.
-template <int DT>
-int dx_cluster(long long tiles, int want) {
-  constexpr int smem = sp24::FfnCfg<DT, sp24::kFfnDx>::SMEM_BYTES;
-  static std::atomic<bool> attr_set[kMaxDevices];
-  auto kern = sp24::ffn_dx_split_kernel<DT>;
-  if (ensure_kernel_attrs(kern, attr_set, smem) != SP24_OK) return 1;
-  return resident_splits<sp24::ffn_dx_split_kernel<DT>>(sp24::kPairThreads, smem, tiles, 2, want);
+  // Few tiles and a long sum: K split over the pairs of a cluster, eight stages a
+  // slice at least (1199 x 3704, f = 744, 30 tiles: 29.3 -> 19.7 us; 300 x 1000, f =
+  // 776: 13.0 -> 10.8; slices of four stages gain nothing more).
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  const int want =
+      static_cast<int>(std::min<long long>({c.sm_count / 2 / tiles, sp24::kFfnMaxSplits, p.k_stages / 8}));
+  return launch_ffn_split<DT, sp24::kFfnForward>(c, a, b, p, want);
 }
 
 template <int DT>
@@ -530,13 +537,14 @@ sp24_status ffn_backward(const FfnCall& c, const sp24_ffn_desc* d, const sp24_ff
     // 35.4 us with four pairs, 11.7 with 48 slices; 64 x 4096, f = 14336 keeps four).
     const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
     const int slices = dx_slices(d->t, d->h, d->f);
-    const int want = static_cast<int>(std::min<long long>({c.sm_count / 2 / tiles, sp24::kMaxDxSplits, p.k_stages}));
-    p.splits = slices > 0 ? slices : want > 1 ? dx_cluster<DT>(tiles, want) : 1;
+    const int want = static_cast<int>(std::min<long long>({c.sm_count / 2 / tiles, sp24::kFfnMaxSplits, p.k_stages}));
     if (slices > 0) {
+      p.splits = slices;
       p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(g->workspace) + dgu_bytes(d->t, d->f));
       p.ld_partial = ffn_ld(d->h);
     }
-    st = slices == 0 && p.splits > 1 ? launch_dx_split<DT>(c, a, b, p) : launch_ffn_pair<DT, sp24::kFfnDx>(c, a, b, p);
+    st = slices > 0 ? launch_ffn_pair<DT, sp24::kFfnDx>(c, a, b, p)
+                    : launch_ffn_split<DT, sp24::kFfnDx>(c, a, b, p, want);
     if (st != SP24_OK) return st;
     if (slices > 0) {
       const long long runs = static_cast<long long>(d->t) * ((d->h + 7) / 8);

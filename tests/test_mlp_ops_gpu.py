@@ -376,7 +376,8 @@ def check_ffn(x, wg, wu, dh, act, out, grads=None):
                                    (65, 128, 128), (100, 264, 1032), (128, 256, 256), (129, 512, 136), (257, 320, 512),
                                    (300, 1000, 776), (513, 256, 1024),
                                    (1300, 1280, 264), (1030, 1000, 136), (2600, 264, 512),
-                                   (33, 72, 14336), (100, 264, 15000), (129, 200, 18888), (256, 64, 16384)])
+                                   (33, 72, 14336), (100, 264, 15000), (129, 200, 18888), (256, 64, 16384),
+                                   (300, 2056, 400), (700, 1032, 264), (1200, 1544, 744)])
 def test_ffn_sizes(t, h, f, dtype, act):
     x, wg, wu, dh = ffn_inputs(t, h, f, dtype, seed=t + h)
     out, saved = sp24.ffn_gated(x, wg, wu, act=act, save=True)
