@@ -160,6 +160,20 @@ def test_rows_zero_tiny_and_not_finite(cols, qdtype):
     assert s[1] == 0 and all(torch.isnan(s[bad]) for bad in (2, 3, 4))
 
 
+def test_norm_whose_squares_leave_fp32():
+    """Sums of squares past fp32's range are flagged, not turned into zeroes."""
+    x = randn(4, 512, seed=1, dtype=torch.bfloat16)
+    x[1] = x[1] * 2.0 ** 90
+    x[2] = x[2] * 2.0 ** -90
+    w = torch.ones(512, device=DEV, dtype=torch.bfloat16)
+    q, s = sp24.rmsnorm_quant(x, w, eps=0.0)
+    assert torch.isnan(s[1]) and torch.isnan(s[2]) and torch.all(q[1:3] == 0)
+    keep = [0, 3]
+    check_rows(q[keep], s[keep], rmsnorm64(x[keep], w, None, 0.0)[1], sp24.I8, scale_tol(512))
+    q, s = sp24.rmsnorm_quant(x, w, eps=1e-6)      # tiny rows are eps's business
+    check_rows(q[[2]], s[[2]], rmsnorm64(x[[2]], w, None, 1e-6)[1], sp24.I8, scale_tol(512))
+
+
 def test_rows_no_rows_and_streams():
     q, s, r = sp24.rmsnorm_quant(torch.empty(0, 64, device=DEV, dtype=torch.bfloat16),
                                  torch.ones(64, device=DEV, dtype=torch.bfloat16),
