@@ -233,7 +233,8 @@ sp24_status sp24_gemm_noalloc(const sp24_gemm_desc* d, sp24_stream_t stream);
    128 columns; any N). */
 typedef enum sp24_activation {
   SP24_ACT_NONE = 0,
-  SP24_ACT_SILU = 1
+  SP24_ACT_SILU = 1,
+  SP24_ACT_GELU_TANH = 2      /* sp24_ffn_* only */
 } sp24_activation;
 
 typedef struct sp24_epilogue {
@@ -337,7 +338,8 @@ sp24_status sp24_gemm_scaled(const sp24_scaled_desc* d, sp24_stream_t stream);
 typedef struct sp24_ffn_desc {
   sp24_dtype dtype;            /* SP24_F16 or SP24_BF16: every tensor below */
   int t, h, f;                 /* tokens (>= 0), input width, intermediate width */
-  sp24_activation act;         /* SP24_ACT_SILU, or SP24_ACT_NONE: g * u */
+  sp24_activation act;         /* SP24_ACT_SILU; SP24_ACT_GELU_TANH: 0.5 g (1 + tanh(sqrt(2 / pi)
+                                  (g + 0.044715 g^3))); SP24_ACT_NONE: g */
   const void* x;               /* t x h */
   int64_t ldx;
   const void* w_gate;          /* f x h */

@@ -58,7 +58,7 @@ struct FfnParams {
   int vec_out;             // 2: rows start on 32 bytes, 1: on 16, 0: neither
   float* saved;            // forward: planes g and u, m x ld_saved each, or null
   long long ld_saved;
-  int silu;
+  int act;
   int* status;
   unsigned long long timeout_ns;
 };
@@ -154,9 +154,40 @@ SP24_DEV void store_run32_f32(float* out, long long ld, uint32_t (&u)[32], int r
   }
 }
 
-// The approximate quotient: the IEEE division takes its slow path for the zeroes
-// of absent rows (255 x 64, f = 128, one tile less a row: 16.3 -> 6.1 us).
-SP24_DEV float gate_act(float g, int silu_on) { return silu_on ? silu_of(g) : g; }
+// Activations of the gate (sp24_activation).  Both are g times a sigmoid: silu of g
+// itself, the tanh form of gelu of k(g) = sqrt(8 / pi) (g + 0.044715 g^3), since
+// (1 + tanh z) / 2 = sigmoid(2 z).  The quotient is the approximate one: the IEEE
+// division takes its slow path for the zeroes of absent rows (255 x 64, f = 128,
+// one tile less a row: 16.3 -> 6.1 us).
+enum : int { kGateNone = 0, kGateSilu = 1, kGateGelu = 2 };
+constexpr float kGeluC = 1.5957691216057308f, kGeluA = 0.044715f;
+
+SP24_DEV float gate_act(float g, int act) {
+  if (act == kGateSilu) return silu_of(g);
+  if (act == kGateGelu) return g * sigmoid_of(kGeluC * g * fmaf(kGeluA * g, g, 1.0f));
+  return g;
+}
+
+// The activation and its derivative: with s = sigmoid(k), a = g s and
+// a' = s + g s (1 - s) k'.
+SP24_DEV void gate_act_grad(float g, int act, float& a, float& da) {
+  if (act == kGateNone) {
+    a = g;
+    da = 1.0f;
+    return;
+  }
+  float k = g, dk = 1.0f, gc = g;
+  if (act == kGateGelu) {
+    // Beyond +-30 the sigmoid is 0 or 1 and g^2 must not overflow into 0 * inf.
+    gc = g > 30.0f ? 30.0f : g < -30.0f ? -30.0f : g;
+    const float q = kGeluA * gc * gc;
+    k = kGeluC * gc * (1.0f + q);
+    dk = kGeluC * fmaf(3.0f, q, 1.0f);
+  }
+  const float s = sigmoid_of(k);
+  a = g * s;
+  da = s * fmaf(gc * (1.0f - s), dk, 1.0f);
+}
 
 SP24_DEV void ffn_tile(const FfnParams& P, int t, int& mt, int& nt) {
   const int per_group = P.group_m * P.n_tiles;
@@ -404,7 +435,7 @@ SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, co
             float h[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              h[e] = gate_act(__uint_as_float(r0[j + e]), P.silu) * __uint_as_float(r1[j + e]);
+              h[e] = gate_act(__uint_as_float(r0[j + e]), P.act) * __uint_as_float(r1[j + e]);
             pk[(c * 32 + j) / 2] = pack16<DT>(h[0], h[1]);
           }
           if (P.saved != nullptr) {
@@ -465,8 +496,8 @@ SP24_DEV void ffn_pair_body(const CUtensorMap& tmA0, const CUtensorMap& tmA1, co
           *reinterpret_cast<float4*>(g) = a;
           *reinterpret_cast<float4*>(g + P.m * P.ld_saved) = u;
         }
-        a = make_float4(gate_act(a.x, P.silu) * u.x, gate_act(a.y, P.silu) * u.y, gate_act(a.z, P.silu) * u.z,
-                        gate_act(a.w, P.silu) * u.w);
+        a = make_float4(gate_act(a.x, P.act) * u.x, gate_act(a.y, P.act) * u.y, gate_act(a.z, P.act) * u.z,
+                        gate_act(a.w, P.act) * u.w);
       }
       if (row >= P.m) continue;
       uint16_t* dst = static_cast<uint16_t*>(P.out0) + row * P.ld_out0 + col;
@@ -563,7 +594,7 @@ __global__ void __launch_bounds__(256)
 template <int DT, int VEC>
 __global__ void __launch_bounds__(256)
     ffn_dgate_kernel(int t, int f, const float* __restrict__ saved, long long ld,
-                     const void* __restrict__ d_out, long long ldd, int silu_on,
+                     const void* __restrict__ d_out, long long ldd, int act,
                      uint16_t* __restrict__ dgu) {
   griddep_launch_dependents();
   griddep_wait();
@@ -593,9 +624,10 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float x = g[j + e];
-        const float sg = __fdividef(1.0f, 1.0f + __expf(-x));
-        du[e] = d[j + e] * (silu_on ? x * sg : x);
-        dg[e] = d[j + e] * u[j + e] * (silu_on ? sg * (1.0f + x * (1.0f - sg)) : 1.0f);
+        float a, da;
+        gate_act_grad(x, act, a, da);
+        du[e] = d[j + e] * a;
+        dg[e] = d[j + e] * u[j + e] * da;
       }
       og[j / 2] = pack16<DT>(dg[0], dg[1]);
       ou[j / 2] = pack16<DT>(du[0], du[1]);

@@ -190,7 +190,7 @@ int dx_slices(int t, int h, int f) {
 sp24_status check_ffn(const sp24_ffn_desc* d) {
   if (d == nullptr) return SP24_ERR_ARG;
   if (!is_16bit(d->dtype)) return SP24_ERR_ARG;
-  if (d->act != SP24_ACT_SILU && d->act != SP24_ACT_NONE) return SP24_ERR_ARG;
+  if (d->act != SP24_ACT_SILU && d->act != SP24_ACT_GELU_TANH && d->act != SP24_ACT_NONE) return SP24_ERR_ARG;
   if (d->t < 0 || d->h <= 0 || d->f <= 0) return SP24_ERR_SHAPE;
   const int64_t ldx = stride_or(d->ldx, d->h), ldg = stride_or(d->ld_gate, d->h),
                 ldu = stride_or(d->ld_up, d->h);
@@ -447,7 +447,7 @@ sp24_status ffn_forward_few(const FfnCall& c, const sp24_ffn_desc* d, void* out,
   p.m_blocks = (d->f + 127) / 128;
   p.out = out, p.ldo = ld_out, p.out_type = DT;
   p.saved = static_cast<float*>(d->saved), p.ld_saved = ffn_ld(d->f);
-  p.silu = d->act == SP24_ACT_SILU;
+  p.act = d->act;
   p.static_weights = static_weights();
   if (pairs) {
     return few_pair_bn(d->t) == 64 ? launch_few_pair<DT, 64>(c, a, a2, b, p)
@@ -494,7 +494,7 @@ sp24_status ffn_forward(const FfnCall& c, const sp24_ffn_desc* d, void* out, int
   p.group_m = 16;
   p.out0 = out, p.ld_out0 = ld_out, p.vec_out = out_vec(out, ld_out);
   p.saved = static_cast<float*>(d->saved), p.ld_saved = ffn_ld(d->f);
-  p.silu = d->act == SP24_ACT_SILU;
+  p.act = d->act;
   // Few tiles and a long sum: K split over the pairs of a cluster, eight stages a
   // slice at least (1199 x 3704, f = 744, 30 tiles: 29.3 -> 19.7 us; 300 x 1000, f =
   // 776: 13.0 -> 10.8; slices of four stages gain nothing more).
@@ -516,7 +516,7 @@ sp24_status ffn_backward(const FfnCall& c, const sp24_ffn_desc* d, const sp24_ff
   sp24_status st = launch_gemm_kernel(kern, grid, 256, 0, c.stream, 0, true, d->t, d->f,
                                       static_cast<const float*>(d->saved), static_cast<long long>(ldw),
                                       static_cast<const void*>(g->d_out), static_cast<long long>(ldd),
-                                      d->act == SP24_ACT_SILU ? 1 : 0, dg);
+                                      static_cast<int>(d->act), dg);
   if (st != SP24_OK) return st;
   CUtensorMap a[2], b[2];
   if (g->dx != nullptr) {

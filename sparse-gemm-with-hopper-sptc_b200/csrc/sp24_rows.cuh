@@ -127,16 +127,17 @@ SP24_DEV uint32_t pack16(float lo, float hi) {
   }
 }
 
-// x sigmoid(x) = x / (1 + 2^(-x log2 e)), the reciprocal and the power each to
+// sigmoid(x) = 1 / (1 + 2^(-x log2 e)), the reciprocal and the power each to
 // about two ulp: beside the 8-bit step that cannot be seen, and the IEEE
 // division made the SwiGLU compute-bound.  Far below zero the power is infinite
-// and the result -0 (true size < 1e-36); -infinity gives NaN, as the formula does.
-SP24_DEV float silu_of(float v) {
+// and the result 0 (true size < 1e-37).
+SP24_DEV float sigmoid_of(float v) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return v * r;
+  return r;
 }
+SP24_DEV float silu_of(float v) { return v * sigmoid_of(v); }   // -infinity: NaN, as the formula
 
 // What the threads of a row agree on.
 struct RowStats {

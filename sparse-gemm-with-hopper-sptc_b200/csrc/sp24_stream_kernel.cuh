@@ -53,7 +53,7 @@ struct StreamParams {
   int out_type;             // 0 f16, 1 bf16, 2 f32
   float* saved;             // ffn: planes of n x ld_saved, or null
   long long ld_saved;
-  int silu;
+  int act;
   int static_weights;       // weights are not written by in-flight work: their first
                             // ring of loads may precede the wait for it
   int* status;
@@ -144,7 +144,7 @@ SP24_DEV float stream_value(const StreamParams& P, uint32_t s0, uint32_t s1, flo
                             float scale_n) {
   if constexpr (OP == kStreamI8) return fmaf(static_cast<float>(static_cast<int>(s0)), scale_m * scale_n, bias);
   else if constexpr (OP == kStreamE4M3) return fmaf(__uint_as_float(s0), scale_m * scale_n, bias);
-  else return gate_act(__uint_as_float(s0), P.silu) * __uint_as_float(s1);
+  else return gate_act(__uint_as_float(s0), P.act) * __uint_as_float(s1);
 }
 
 template <int OP>
@@ -603,7 +603,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
               P.saved[(P.n + tok) * P.ld_saved + row] = __uint_as_float(u[j]);
             }
             store16<DT>(P.out, tok * P.ldo + row,
-                        gate_act(__uint_as_float(g[j]), P.silu) * __uint_as_float(u[j]));
+                        gate_act(__uint_as_float(g[j]), P.act) * __uint_as_float(u[j]));
           }
         }
       }

@@ -52,6 +52,7 @@ MAX_PEERS = 7
 HINT_NONE, HINT_STATIC_WEIGHTS = 0, 1
 
 ACT_NONE, ACT_SILU = 0, 1
+ACT_GELU_TANH = 2   # ffn_gated only
 
 
 class Sp24Error(RuntimeError):
@@ -598,8 +599,9 @@ def _ffn_forward(s, x, w_gate, w_up, act, save):
 
 
 def ffn_gated(x, w_gate, w_up, *, act=ACT_SILU, save=False, stream=None):
-    """sp24_ffn_forward: act(x w_gate^T) * (x w_up^T) -> [t, f]; with save=True
-    also the opaque buffer that ffn_gated_backward takes."""
+    """sp24_ffn_forward: act(x w_gate^T) * (x w_up^T) -> [t, f], act one of
+    ACT_SILU, ACT_GELU_TANH and ACT_NONE; with save=True also the opaque buffer
+    that ffn_gated_backward takes."""
     return _on(_same_device(x, w_gate, w_up), stream, _ffn_forward, x, w_gate, w_up, act, save)
 
 

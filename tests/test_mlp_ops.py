@@ -75,7 +75,7 @@ FFN = dict(dtype=1, t=4, h=64, f=96, act=1, x=P, w_gate=P, w_up=P)
 
 
 @pytest.mark.parametrize("kw,code", [
-    (dict(dtype=2), 8), (dict(dtype=7), 8), (dict(act=2), 8),
+    (dict(dtype=2), 8), (dict(dtype=7), 8), (dict(act=3), 8), (dict(act=-1), 8),
     (dict(t=-1), 1), (dict(h=0), 1), (dict(f=0), 1),
     (dict(ldx=63), 1), (dict(ld_gate=56), 1), (dict(ld_up=8), 1),
     (dict(x=None), 8), (dict(w_gate=None), 8), (dict(w_up=None), 8),
@@ -136,6 +136,17 @@ def test_plain_gemm_still_refuses_the_new_types():
         assert lib.sp24_prune_2of4(dtype, P, 8, 8, 0, P, 0, None) == 8
     assert lib.sp24_repack_meta(sp24.F32, P, 64, 64, P, None) == 8
     assert lib.sp24_repack_meta(sp24.I8, P, 64, 32, P, None) == 1    # k % 64 as for fp8
+
+
+def test_fused_gemm_still_refuses_the_new_activation():
+    lib = sp24.load()
+    d = sp24.GemmDesc()
+    d.m = d.n = d.k = 128
+    d.a_c = d.meta = d.b = d.c_f32 = P
+    d.meta_format = sp24.META_TC
+    e = sp24.Epilogue()
+    e.act = sp24.ACT_GELU_TANH
+    assert lib.sp24_gemm_fused(ctypes.byref(d), ctypes.byref(e), None) == 8
 
 
 def test_shim_refusals():

@@ -339,7 +339,15 @@ def ffn64(x, wg, wu, act):
     x, wg, wu = x.double(), wg.double(), wu.double()
     g, u = x @ wg.t(), x @ wu.t()
     s = torch.sigmoid(g)
-    a, da = (g * s, s * (1 + g * (1 - s))) if act == sp24.ACT_SILU else (g, torch.ones_like(g))
+    if act == sp24.ACT_SILU:
+        a, da = g * s, s * (1 + g * (1 - s))
+    elif act == sp24.ACT_GELU_TANH:
+        c = (2 / torch.pi) ** 0.5
+        t = torch.tanh(c * (g + 0.044715 * g ** 3))
+        a = 0.5 * g * (1 + t)
+        da = 0.5 * (1 + t) + 0.5 * g * (1 - t * t) * c * (1 + 3 * 0.044715 * g * g)
+    else:
+        a, da = g, torch.ones_like(g)
     return g, u, a, da
 
 
@@ -355,8 +363,10 @@ def check_ffn(x, wg, wu, dh, act, out, grads=None):
     g64, u64, a, da = ffn64(x, wg, wu, act)
     X, WG, WU = x.double().abs(), wg.double().abs(), wu.double().abs()
     eg, eu = (h + 8) * E * (X @ WG.t()), (h + 8) * E * (X @ WU.t())   # of the sums g and u
-    # |act'| <= 1.1, |act''| <= 0.5; the activation's own fp32 error is 16 e
-    eh = 1.1 * eg * (u64.abs() + eu) + (a.abs() + 1.1 * eg) * eu + 16 * E * (a * u64).abs()
+    # |act'| <= 1.1 and |act''| <= 0.5 for silu, 1.13 and 0.8 for gelu; the
+    # activation's own fp32 error is 16 e
+    d1, d2 = (1.13, 0.8) if act == sp24.ACT_GELU_TANH else (1.1, 0.5)
+    eh = d1 * eg * (u64.abs() + eu) + (a.abs() + d1 * eg) * eu + 16 * E * (a * u64).abs()
     y = a * u64
     err = (out.double() - y).abs()
     assert torch.all(err <= u * y.abs() * (1 + 1e-3) + 1.01 * eh + tiny)
@@ -365,8 +375,8 @@ def check_ffn(x, wg, wu, dh, act, out, grads=None):
         return
     D = dh.double()
     dg, du = D * u64 * da, D * a
-    edg = D.abs() * (0.5 * eg * (u64.abs() + eu) + 1.1 * eu + 16 * E * u64.abs()) + u * dg.abs() * 1.01 + tiny
-    edu = D.abs() * (1.1 * eg + 16 * E * a.abs()) + u * du.abs() * 1.01 + tiny
+    edg = D.abs() * (d2 * eg * (u64.abs() + eu) + d1 * eu + 16 * E * u64.abs()) + u * dg.abs() * 1.01 + tiny
+    edu = D.abs() * (d1 * eg + 16 * E * a.abs()) + u * du.abs() * 1.01 + tiny
     dx, dwg, dwu = grads
     S = (dg.abs() + edg) @ WG + (du.abs() + edu) @ WU
     for got, want, tol in (
@@ -446,6 +456,19 @@ def test_ffn_strides_padding_and_partial_gradients(t):
         assert torch.equal(b[:, :h], want) and torch.all(b[:, h:] == 9)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,h,f", [(1, 64, 136), (40, 264, 14336), (90, 512, 256), (200, 1024, 264), (300, 320, 512),
+                                   (1100, 128, 2000)])
+def test_ffn_gelu(t, h, f, dtype):
+    """The tanh form of gelu through every forward kernel, and its gradients."""
+    x, wg, wu, dh = ffn_inputs(t, h, f, dtype, seed=t)
+    x[0] *= 40                       # gates far into both tails
+    out, saved = sp24.ffn_gated(x, wg, wu, act=sp24.ACT_GELU_TANH, save=True)
+    grads = sp24.ffn_gated_backward(dh, x, wg, wu, saved, act=sp24.ACT_GELU_TANH)
+    check_ffn(x, wg, wu, dh, sp24.ACT_GELU_TANH, out, grads)
+    check_ffn(x, wg, wu, dh, sp24.ACT_GELU_TANH, sp24.ffn_gated(x, wg, wu, act=sp24.ACT_GELU_TANH))
+
+
 def test_ffn_no_tokens():
     _, wg, wu, _ = ffn_inputs(1, 64, 96, torch.bfloat16)
     x, dh = (torch.empty(0, n, device=DEV, dtype=torch.bfloat16) for n in (64, 96))
@@ -474,7 +497,7 @@ def test_ffn_extreme_gates():
     assert torch.isnan(dwg[:, 0]).all() and torch.isnan(dwu[:, 0]).all()
 
 
-@pytest.mark.parametrize("act", [sp24.ACT_SILU, sp24.ACT_NONE])
+@pytest.mark.parametrize("act", [sp24.ACT_SILU, sp24.ACT_GELU_TANH, sp24.ACT_NONE])
 def test_ffn_gradients_against_differences(act):
     """Directional derivatives of the 64-bit formula by central differences
     (error eps^2 / 6 of the third derivative, about 1e-9 here), against the
