@@ -588,8 +588,9 @@ __global__ void __launch_bounds__(256)
 // dg = d_out u act'(g) and du = d_out act(g) from the saved fp32 sums, rounded
 // to 16 bits: eight columns a thread, rows of ld (a multiple of 8) elements.
 // Bound by HBM: 14 bytes an element (4096 x 14336: 822 MB in 126 us, 6.5 TB/s).
-// The padding past column f is written too (its inputs are whatever the buffer
-// holds) and never read: the products' tensor maps end at f.
+// Only the units of eight that hold a column below f are walked: d_out has no
+// padding to read, and the products' tensor maps end at f.  A last unit past f is
+// written whole (the saved sums there are whatever the buffer holds).
 // VEC: d_out's rows start on 16 bytes and f is a multiple of 8.
 template <int DT, int VEC>
 __global__ void __launch_bounds__(256)
@@ -598,7 +599,7 @@ __global__ void __launch_bounds__(256)
                      uint16_t* __restrict__ dgu) {
   griddep_launch_dependents();
   griddep_wait();
-  const long long per_row = ld / 8, total = per_row * t, plane = ld * t;
+  const long long per_row = (f + 7) / 8, total = per_row * t, plane = ld * t;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
     const long long row = i / per_row;
     const int col = static_cast<int>(i - row * per_row) * 8;

@@ -509,7 +509,7 @@ sp24_status ffn_backward(const FfnCall& c, const sp24_ffn_desc* d, const sp24_ff
   const int64_t ldw = ffn_ld(d->f), ldd = stride_or(g->ld_d_out, d->f);
   uint16_t* dg = static_cast<uint16_t*>(g->workspace);
   uint16_t* du = dg + static_cast<size_t>(d->t) * ldw;
-  const long long chunks = d->t * (ldw / 8);
+  const long long chunks = static_cast<long long>(d->t) * ((d->f + 7) / 8);
   const unsigned grid = static_cast<unsigned>(std::min<long long>((chunks + 255) / 256, c.sm_count * 8));
   const bool vec = aligned16(g->d_out) && ldd % 8 == 0 && d->f % 8 == 0;
   auto kern = vec ? sp24::ffn_dgate_kernel<DT, 1> : sp24::ffn_dgate_kernel<DT, 0>;

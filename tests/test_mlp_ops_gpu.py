@@ -687,3 +687,32 @@ def test_inputs_freed_right_after_a_call_on_another_stream():
         side.synchronize()
         assert all(torch.equal(q, want[0]) and torch.equal(s, want[1]) for q, s in big)
         del junk
+
+
+@pytest.mark.parametrize("t,f", [(1, 8), (3, 72), (5, 264), (70, 776), (4, 51), (2, 128)])
+def test_ffn_backward_touches_no_column_past_f(t, f):
+    """dg and du are formed from the columns of d_out that exist: what the
+    workspace holds past them stays as it was (units of eight columns, rows of
+    64), and NaN beside d_out's rows reaches no gradient."""
+    h, ld = 64, (f + 63) // 64 * 64
+    x, wg, wu, dh = ffn_inputs(t, h, f, torch.float16, seed=f)
+    out, saved = sp24.ffn_gated(x, wg, wu, save=True)
+    wide = torch.full((t, f + 64), float("nan"), device=DEV, dtype=torch.float16)
+    wide[:, :f] = dh
+    lib, stream = sp24.load(), torch.cuda.current_stream().cuda_stream
+    d = sp24.FfnDesc()
+    d.dtype, d.t, d.h, d.f, d.act = sp24.F16, t, h, f, sp24.ACT_SILU
+    d.x, d.w_gate, d.w_up = x.data_ptr(), wg.data_ptr(), wu.data_ptr()
+    d.saved, d.saved_bytes = saved.data_ptr(), saved.numel()
+    size = lib.sp24_ffn_workspace_bytes(t, h, f)
+    for d_out, ldd in ((dh, f), (wide, f + 64)):
+        ws = torch.full((size // 2,), 0x5A5A, device=DEV, dtype=torch.int16)
+        dx, dwg, dwu = (torch.empty(r, h, device=DEV, dtype=torch.float16) for r in (t, f, f))
+        g = sp24.FfnGrads()
+        g.d_out, g.ld_d_out = d_out.data_ptr(), ldd
+        g.dx, g.dw_gate, g.dw_up = (v.data_ptr() for v in (dx, dwg, dwu))
+        g.workspace, g.workspace_bytes = ws.data_ptr(), size
+        assert lib.sp24_ffn_backward(ctypes.byref(d), ctypes.byref(g), stream) == 0
+        check_ffn(x, wg, wu, dh, sp24.ACT_SILU, out, (dx, dwg, dwu))
+        planes = ws[:2 * t * ld].view(2, t, ld)
+        assert torch.all(planes[:, :, (f + 7) // 8 * 8:] == 0x5A5A)
