@@ -175,3 +175,42 @@ def test_packed_descriptors_match_the_structures():
         assert len(got) <= ctypes.sizeof(cls)
         back = cls.from_buffer_copy(got.ljust(ctypes.sizeof(cls), b"\0"))
         assert [getattr(back, n) for n, _ in cls._fields_] == [getattr(want, n) for n, _ in cls._fields_]
+
+
+@pytest.mark.parametrize("step,aligned", [(64, True), (72, False), (65, False)])
+def test_copied_weights_lose_the_static_hint(monkeypatch, step, aligned):
+    """Weights that the shim copies on the stream are in-flight work of the
+    call: it is launched without the hint, and the caller's hint stays set."""
+    real, seen = sp24.load(), []
+
+    class Library:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def sp24_gemm_scaled(self, *args):
+            seen.append(real.sp24_get_launch_hints())
+            return 0
+
+        sp24_ffn_forward = sp24_gemm_scaled
+
+    monkeypatch.setattr(sp24, "_lib", Library())
+    a_c = torch.zeros(128, step, dtype=torch.int8)[:, :64]
+    x8 = torch.zeros(4, 128, dtype=torch.int8)
+    image = torch.zeros(sp24.meta_tc_bytes(128, 128), dtype=torch.uint8)
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    w = torch.zeros(96, 64, dtype=torch.bfloat16)
+    odd = torch.zeros(96, 64 if aligned else 65, dtype=torch.bfloat16)[:, :64]
+    for hints in (sp24.HINT_NONE, sp24.HINT_STATIC_WEIGHTS):
+        sp24.set_launch_hints(hints)
+        try:
+            sp24._gemm_scaled(0, a_c, image, x8, None, None, None, None)
+            sp24._ffn_forward(0, x, w, odd, sp24.ACT_SILU, False)
+            sp24._ffn_forward(0, x, odd, w, sp24.ACT_SILU, False)
+            assert sp24.get_launch_hints() == hints
+        finally:
+            sp24.set_launch_hints(sp24.HINT_NONE)
+        # tokens may be copied: they are loaded after the wait in any case
+        sp24._ffn_forward(0, torch.zeros(4, 65, dtype=torch.bfloat16)[:, :64], w, w, sp24.ACT_SILU, False)
+        want = hints if aligned else sp24.HINT_NONE
+        assert seen == [want, want, want, sp24.HINT_NONE]
+        seen.clear()

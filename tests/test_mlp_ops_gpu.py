@@ -716,3 +716,29 @@ def test_ffn_backward_touches_no_column_past_f(t, f):
         check_ffn(x, wg, wu, dh, sp24.ACT_SILU, out, (dx, dwg, dwu))
         planes = ws[:2 * t * ld].view(2, t, ld)
         assert torch.all(planes[:, :, (f + 7) // 8 * 8:] == 0x5A5A)
+
+
+@pytest.mark.parametrize("n", [1, 60, 300])
+def test_static_weight_hint_with_weights_that_are_copied(n):
+    """Under the hint, weights whose rows are off the 16-byte grid: the shim's
+    copies are made just before each product, over memory that held others."""
+    h, f, m, k = 1004, 520, 300, 256
+    x = randn(n, h, seed=1, dtype=torch.bfloat16)
+    pairs = [[randn(f, h, seed=10 * i + j, std=0.02, dtype=torch.bfloat16) for j in (2, 3)] for i in range(3)]
+    packed = [weights_2of4(m, k, sp24.I8, seed=i)[:2] for i in range(3)]
+    odd = [torch.zeros(m, k // 2 + 4, device=DEV, dtype=torch.int8)[:, :k // 2].copy_(a) for a, _ in packed]
+    q = tokens_8bit(n, k, sp24.I8, seed=4)
+
+    def products():
+        return [(sp24.ffn_gated(x, *w), sp24.gemm_scaled(a, image, q, out_dtype=torch.float32))
+                for w, a, (_, image) in zip(pairs, odd, packed)]
+
+    want = products()
+    torch.cuda.synchronize()
+    sp24.set_launch_hints(sp24.HINT_STATIC_WEIGHTS)
+    try:
+        for _ in range(5):
+            assert all(torch.equal(a, b) for p, r in zip(products(), want) for a, b in zip(p, r))
+        assert sp24.get_launch_hints() == sp24.HINT_STATIC_WEIGHTS
+    finally:
+        sp24.set_launch_hints(sp24.HINT_NONE)
