@@ -466,12 +466,16 @@ _codes = {}
 
 
 def _code_tables():
-    """Torch dtype -> library code, by use."""
+    """Torch dtype -> library code, by use.  Published whole: another thread sees
+    no table or all of them."""
+    global _codes
     import torch
-    _codes["16"] = {torch.float16: F16, torch.bfloat16: BF16}
-    _codes["8"] = {torch.int8: I8, torch.float8_e4m3fn: E4M3}
-    _codes["out"] = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
-    _codes["of_8"] = {I8: torch.int8, E4M3: torch.float8_e4m3fn}
+    _codes = {
+        "16": {torch.float16: F16, torch.bfloat16: BF16},
+        "8": {torch.int8: I8, torch.float8_e4m3fn: E4M3},
+        "out": {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32},
+        "of_8": {I8: torch.int8, E4M3: torch.float8_e4m3fn},
+    }
     return _codes
 
 

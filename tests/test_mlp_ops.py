@@ -1,6 +1,7 @@
 """The MLP-block operators without a GPU: what their descriptors refuse before
 any CUDA call, their buffer sizes, and what the torch-facing shim refuses."""
 import ctypes
+import sys
 
 import pytest
 import torch
@@ -214,3 +215,59 @@ def test_copied_weights_lose_the_static_hint(monkeypatch, step, aligned):
         want = hints if aligned else sp24.HINT_NONE
         assert seen == [want, want, want, sp24.HINT_NONE]
         seen.clear()
+
+
+def test_type_tables_are_published_whole(monkeypatch):
+    """What another thread finds at every line of the first call that builds the
+    tables: nothing, or all of them."""
+    whole = set(sp24._code_tables())
+    monkeypatch.setattr(sp24, "_codes", {})
+    seen = []
+
+    def trace(frame, event, arg):
+        if frame.f_code is sp24._code_tables.__code__:
+            seen.append(set(sp24._codes))
+            return trace
+
+    before = sys.gettrace()
+    sys.settrace(trace)
+    try:
+        sp24._code_tables()
+    finally:
+        sys.settrace(before)
+    assert len(seen) > 2 and all(s in (set(), whole) for s in seen) and set(sp24._codes) == whole
+
+
+def test_first_calls_from_several_threads_in_a_fresh_process():
+    """Threads whose very first calls meet: each gets its own refusal (tensors
+    without a GPU), past the type tables."""
+    import os
+    import subprocess
+    code = """
+import sys, threading
+sys.path.insert(0, sys.argv[1])
+sys.setswitchinterval(1e-6)
+import torch
+import sp24
+x = torch.zeros(4, 64, dtype=torch.bfloat16)
+x8, image = torch.zeros(4, 128, dtype=torch.int8), torch.zeros(4096, dtype=torch.uint8)
+gate, failed = threading.Barrier(8), []
+def first(i):
+    gate.wait()
+    for call in (lambda: sp24._ffn_args(x, x, x, sp24.ACT_SILU),
+                 lambda: sp24._gemm_scaled(0, x8.float(), image, x8, None, None, None, None),
+                 lambda: sp24._rows_quant(0, "sp24_quantize_rows", x.float(), sp24.I8, None, None, None, 0.0)):
+        try:
+            call()
+        except ValueError:
+            pass
+        except Exception as e:
+            failed.append(repr(e))
+for _ in range(50):
+    sp24._codes = {}
+    threads = [threading.Thread(target=first, args=(i,)) for i in range(8)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+assert not failed, failed
+"""
+    subprocess.run([sys.executable, "-c", code, os.path.dirname(sp24.__file__)], check=True, timeout=300)
