@@ -263,9 +263,9 @@ sp24_status sp24_gemm_fused(const sp24_gemm_desc* d, const sp24_epilogue* e,
      amax = max |y|,  scale = amax / Q,  q = round(y * Q / amax),  Q = 127 (SP24_I8)
      or 448 (SP24_E4M3); int8 rounds half to even, e4m3 to nearest even.
    A row of zeroes has scale 0 and codes 0.  A row that holds a NaN or an
-   infinity, or whose sum of squares leaves fp32's range (values around 1e18, or
-   below 1e-19 with eps 0), has scale NaN and codes 0, so everything computed from
-   it is NaN.
+   infinity, or whose sum of squares leaves fp32's normal range (values around
+   1e18; a non-zero row with mean(s^2) + eps below 2^-126, i.e. values below 1e-19
+   with eps 0), has scale NaN and codes 0, so everything computed from it is NaN.
      sp24_rmsnorm_quant  s = x + residual (fp32; residual optional; its 16-bit
                          rounding is written to residual_out when given, which
                          may be the residual itself),

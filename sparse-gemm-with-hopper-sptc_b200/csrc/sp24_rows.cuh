@@ -204,8 +204,9 @@ SP24_DEV RowScale row_scale(uint32_t top, float gain) {
   // brought in first.
   r.lift = amax < 1e-30f ? 0x1p100f : amax > 1e30f ? 0x1p-40f : 1.0f;
   const float bounded = amax * r.lift;
-  // A gain of 0 or infinity: the squares left fp32's range (or met a NaN).
-  r.bad = !(bounded < 3e38f) || (top != 0 && !(gain > 0.0f && gain < 3e38f));
+  // A gain of 0: the squares overflowed; NaN: they met one; above 2^63: their mean
+  // is below fp32's normal range, and the subnormal sum has lost digits.
+  r.bad = !(bounded < 3e38f) || (top != 0 && !(gain > 0.0f && gain <= 0x1p63f));
   r.inv = (r.bad || top == 0) ? 0.0f : __fdividef(Q, bounded);
   r.scale = r.bad ? __uint_as_float(0x7FC00000u) : top == 0 ? 0.0f : amax * gain * (1.0f / Q);
   return r;

@@ -742,3 +742,25 @@ def test_static_weight_hint_with_weights_that_are_copied(n):
         assert sp24.get_launch_hints() == sp24.HINT_STATIC_WEIGHTS
     finally:
         sp24.set_launch_hints(sp24.HINT_NONE)
+
+
+@pytest.mark.parametrize("cols", [100, 512, 1001, 4096, 40001])
+def test_norm_whose_squares_are_subnormal(cols):
+    """Sums of squares that lose digits below 2^-126 are flagged too, in every
+    form of the kernel; rows just above, and rows whose eps carries the sum, are
+    right to the usual tolerance."""
+    powers = (-60, -62, -65, -69, -72, -73, -75)
+    x = randn(1, cols, seed=1, dtype=torch.bfloat16).repeat(len(powers) + 1, 1)
+    for i, e in enumerate(powers):
+        x[i] = x[i] * 2.0 ** e
+    x[-1] = 0
+    w = (1 + randn(cols, seed=2, std=0.1)).to(torch.bfloat16)
+    mean = x.double().square().mean(dim=1)
+    bad = (mean > 0) & (mean < 2.0 ** -126)
+    assert bad.tolist() == [False, False] + [True] * 5 + [False]
+    q, s = sp24.rmsnorm_quant(x, w, eps=0.0)
+    assert torch.equal(torch.isnan(s), bad) and torch.all(q[bad] == 0) and s[-1] == 0
+    check_rows(q[:2], s[:2], rmsnorm64(x[:2], w, None, 0.0)[1], sp24.I8, scale_tol(cols))
+    eps = 2.0 ** -125
+    q, s = sp24.rmsnorm_quant(x, w, eps=eps)
+    check_rows(q, s, rmsnorm64(x, w, None, eps)[1], sp24.I8, scale_tol(cols))
