@@ -454,6 +454,8 @@ def _on(index, stream, call, *args):
     import torch
     if stream is None and torch._C._cuda_getDevice() == index:
         return call(torch._C._cuda_getCurrentRawStream(index), *args)
+    if stream is not None and stream.device_index != index:
+        raise ValueError(f"a stream of cuda:{stream.device_index} for tensors on cuda:{index}")
     with torch.cuda.device(index), torch.cuda.stream(stream):
         if stream is not None:
             for t in args:

@@ -1,5 +1,6 @@
 """The MLP-block operators without a GPU: what their descriptors refuse before
 any CUDA call, their buffer sizes, and what the torch-facing shim refuses."""
+import contextlib
 import ctypes
 import sys
 
@@ -271,3 +272,22 @@ for _ in range(50):
 assert not failed, failed
 """
     subprocess.run([sys.executable, "-c", code, os.path.dirname(sp24.__file__)], check=True, timeout=300)
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_streams_of_another_device_are_refused(monkeypatch, current):
+    """A named stream has to be one of the tensors' device: entering it would
+    make its own device current, and the launch would go there."""
+    class Stream:
+        device_index = 1
+
+    launched = []
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "stream", lambda stream: contextlib.nullcontext())
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    with pytest.raises(ValueError, match="stream of cuda:1"):
+        sp24._on(0, Stream(), launched.append)
+    assert not launched
+    sp24._on(1, Stream(), launched.append)
+    assert launched == [0]
