@@ -560,7 +560,7 @@ def _gemm_scaled(s, a_c, meta_tc, x, scale_w, scale_x, bias, out_dtype):
                          "both float8_e4m3fn are wanted")
     if out is None:
         raise ValueError(f"gemm_scaled: out_dtype {out_dtype}")
-    given = a_c
+    given = a_c, meta_tc
     a_c, lda = _tma_rows(a_c, "a_c")
     m, k = a_c.shape[0], 2 * a_c.shape[1]
     x, ldx = _tma_rows(x, "x", k)
@@ -568,13 +568,16 @@ def _gemm_scaled(s, a_c, meta_tc, x, scale_w, scale_x, bias, out_dtype):
     image = (m + 255) // 256 * ((k + 127) // 128) * 4096      # sp24_meta_tc_bytes
     if meta_tc.nbytes != image:
         raise ValueError(f"meta_tc: {meta_tc.nbytes} bytes, {image} expected")
+    if not meta_tc.is_contiguous():
+        meta_tc = meta_tc.contiguous()
     scale_w, p_w = _vector_f32(scale_w, m, "scale_w")
     scale_x, p_x = _vector_f32(scale_x, n, "scale_x")
     bias, p_b = _vector_f32(bias, m, "bias")
     c = x.new_empty((n, m), dtype=out_dtype or torch.bfloat16)
     d = _PACK_SCALED(code, out, m, n, k, a_c.data_ptr(), lda, meta_tc.data_ptr(), x.data_ptr(), ldx,
                      p_w, p_x, p_b, c.data_ptr(), 0, 0)
-    _check(_fresh_copies(lib, a_c is not given, lib.sp24_gemm_scaled, d, s), "sp24_gemm_scaled")
+    copied = a_c is not given[0] or meta_tc is not given[1]
+    _check(_fresh_copies(lib, copied, lib.sp24_gemm_scaled, d, s), "sp24_gemm_scaled")
     return c
 
 
@@ -636,6 +639,8 @@ def _ffn_backward(s, d_out, x, w_gate, w_up, saved, act, need_dx, need_dw):
     args, keep = _ffn_args(x, w_gate, w_up, act)
     _, t, h, f = args[:4]
     d_out, ldd = _rows2d(d_out, "d_out", f, t)
+    if not saved.is_contiguous():
+        saved = saved.contiguous()
     dx = x.new_empty((t, h)) if need_dx else None
     dw_gate = dw_up = None
     if need_dw:

@@ -291,3 +291,46 @@ def test_streams_of_another_device_are_refused(monkeypatch, current):
     assert not launched
     sp24._on(1, Stream(), launched.append)
     assert launched == [0]
+
+
+@pytest.mark.parametrize("form", ["plain", "strided", "expanded"])
+def test_strided_images_and_saved_buffers_are_read_as_they_are_indexed(monkeypatch, form):
+    """The metadata image and the saved buffer go to the library as plain bytes:
+    strided ones are copied first, and none is read past its own storage."""
+    real, seen = sp24.load(), []
+
+    class Library:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def sp24_gemm_scaled(self, d, stream):
+            desc = sp24.ScaledDesc.from_buffer_copy(d.ljust(ctypes.sizeof(sp24.ScaledDesc), b"\0"))
+            seen.append((ctypes.string_at(desc.meta, 4096), real.sp24_get_launch_hints()))
+            return 0
+
+        def sp24_ffn_backward(self, d, grads, stream):
+            desc = sp24.FfnDesc.from_buffer_copy(d.ljust(ctypes.sizeof(sp24.FfnDesc), b"\0"))
+            seen.append((ctypes.string_at(desc.saved, desc.saved_bytes), None))
+            return 0
+
+    def strided(v):
+        if form == "strided":
+            wide = torch.zeros(2 * v.numel(), dtype=v.dtype)
+            wide[::2] = v
+            return wide[::2]
+        return v[:1].expand(v.numel()) if form == "expanded" else v
+
+    monkeypatch.setattr(sp24, "_lib", Library())
+    image = strided(torch.randint(0, 256, (4096,), dtype=torch.uint8))
+    sp24.set_launch_hints(sp24.HINT_STATIC_WEIGHTS)
+    try:
+        sp24._gemm_scaled(0, torch.zeros(128, 64, dtype=torch.int8), image, torch.zeros(4, 128, dtype=torch.int8),
+                          None, None, None, None)
+    finally:
+        sp24.set_launch_hints(sp24.HINT_NONE)
+    x, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(96, 64, dtype=torch.bfloat16)
+    saved = strided(torch.randint(0, 256, (real.sp24_ffn_saved_bytes(4, 96),), dtype=torch.uint8))
+    sp24._ffn_backward(0, torch.zeros(4, 96, dtype=torch.bfloat16), x, w, w, saved, sp24.ACT_SILU, True, True)
+    # an image that was copied is in-flight work: the launch goes without the hint
+    hints = sp24.HINT_STATIC_WEIGHTS if form == "plain" else sp24.HINT_NONE
+    assert seen == [(bytes(image.tolist()), hints), (bytes(saved.tolist()), None)]
