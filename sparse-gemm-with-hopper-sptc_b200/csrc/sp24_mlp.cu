@@ -178,12 +178,15 @@ inline int64_t ffn_ld(int f) { return static_cast<int64_t>(round_up(static_cast<
 inline size_t dgu_bytes(int t, int f) { return static_cast<size_t>(t) * 2 * ffn_ld(f) * 2; }
 
 // K slices of a dx tile that go through the workspace: where the tiles are so few
-// that clusters of four pairs would leave most of the 74 idle, as many slices as
-// there are pairs for them, of at least eight stages each; else none.
-int dx_slices(int t, int h, int f) {
+// that clusters of four pairs would leave most of the pairs idle, as many slices as
+// there are pairs for them, of at least eight stages each; else none.  The
+// workspace, whose size is asked for without a device, has room for the slices of a
+// whole B200 (74 pairs); a part with fewer SMs takes fewer.
+constexpr int kMaxPairs = 74;
+int dx_slices(int t, int h, int f, int pairs = kMaxPairs) {
   const long long tiles = ((t + 255LL) / 256) * ((h + 255LL) / 256);
   const long long stages = 2 * ((f + 63LL) / 64);
-  const long long slices = std::min(74 / tiles, stages / 8);
+  const long long slices = std::min(pairs / tiles, stages / 8);
   return slices > sp24::kFfnMaxSplits ? static_cast<int>(slices) : 0;
 }
 
@@ -536,7 +539,7 @@ sp24_status ffn_backward(const FfnCall& c, const sp24_ffn_desc* d, const sp24_ff
     // Very few: split further, through the workspace (40 x 112, f = 12344, one tile:
     // 35.4 us with four pairs, 11.7 with 48 slices; 64 x 4096, f = 14336 keeps four).
     const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
-    const int slices = dx_slices(d->t, d->h, d->f);
+    const int slices = dx_slices(d->t, d->h, d->f, std::min(kMaxPairs, c.sm_count / 2));
     const int want = static_cast<int>(std::min<long long>({c.sm_count / 2 / tiles, sp24::kFfnMaxSplits, p.k_stages}));
     if (slices > 0) {
       p.splits = slices;
