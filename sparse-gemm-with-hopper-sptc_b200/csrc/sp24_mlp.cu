@@ -86,11 +86,18 @@ sp24_status launch_rows_kernel(const sp24::RowsParams& p, const DeviceInfo& di, 
   return launch_gemm_kernel(kern, grid, threads, smem, s, 0, true, p);
 }
 
-template <int DT, int MODE, int I8, int V, int VPT>
+// Rows of more than LO and at most HI vectors, VPT of them a thread; only the
+// forms that such rows reach are built.
+template <int DT, int MODE, int I8, int V, int VPT, int LO, int HI>
 sp24_status launch_rows_vpt(const sp24::RowsParams& p, const DeviceInfo& di, int vecs, cudaStream_t s) {
-  if (vecs <= 32 * VPT) return launch_rows_kernel<DT, MODE, I8, V, VPT, true>(p, di, 256, s);
-  const unsigned threads = static_cast<unsigned>(round_up((vecs + VPT - 1) / VPT, 32));
-  return launch_rows_kernel<DT, MODE, I8, V, VPT, false>(p, di, threads, s);
+  constexpr int kWarp = 32 * VPT;   // vectors that one warp holds
+  if constexpr (LO < kWarp)
+    if (HI <= kWarp || vecs <= kWarp) return launch_rows_kernel<DT, MODE, I8, V, VPT, true>(p, di, 256, s);
+  if constexpr (HI > kWarp) {
+    const unsigned threads = static_cast<unsigned>(round_up((vecs + VPT - 1) / VPT, 32));
+    return launch_rows_kernel<DT, MODE, I8, V, VPT, false>(p, di, threads, s);
+  }
+  return SP24_ERR_SHAPE;   // not reached
 }
 
 // Vectors a thread holds.  The norm waits for a row's two inputs, sum and weight
@@ -106,15 +113,22 @@ sp24_status launch_rows_vpt(const sp24::RowsParams& p, const DeviceInfo& di, int
 template <int DT, int MODE, int I8, int V>
 sp24_status launch_rows_v(const sp24::RowsParams& p, const DeviceInfo& di, cudaStream_t s) {
   const int vecs = (p.cols + V - 1) / V;
-  if constexpr (V == 8) {
-    const bool norm = MODE == sp24::kRowsNorm;
-    if (vecs <= (norm ? 512 : 32)) return launch_rows_vpt<DT, MODE, I8, V, 1>(p, di, vecs, s);
+  if constexpr (V == 8 && MODE == sp24::kRowsNorm) {
+    if (vecs <= 512) return launch_rows_vpt<DT, MODE, I8, V, 1, 0, 512>(p, di, vecs, s);
+    if (vecs <= 2048) return launch_rows_vpt<DT, MODE, I8, V, 2, 512, 2048>(p, di, vecs, s);
+    if (vecs <= 4096) return launch_rows_vpt<DT, MODE, I8, V, 4, 2048, 4096>(p, di, vecs, s);
+  } else if constexpr (V == 8) {
+    if (vecs <= 32) return launch_rows_vpt<DT, MODE, I8, V, 1, 0, 32>(p, di, vecs, s);
     const bool few = p.rows <= 2 * di.sm_count;
-    if ((norm || few) && vecs <= 2 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 2>(p, di, vecs, s);
-    if (vecs <= 4 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 4>(p, di, vecs, s);
+    if (few && vecs <= 2048) return launch_rows_vpt<DT, MODE, I8, V, 2, 32, 2048>(p, di, vecs, s);
+    if (vecs <= 4096) return launch_rows_vpt<DT, MODE, I8, V, 4, 32, 4096>(p, di, vecs, s);
+  } else if constexpr (V == 4) {
+    if (vecs <= 4096) return launch_rows_vpt<DT, MODE, I8, V, 4, 0, 4096>(p, di, vecs, s);
+  } else if constexpr (V == 2) {
+    if (vecs <= 4096) return launch_rows_vpt<DT, MODE, I8, V, 4, 0, 4096>(p, di, vecs, s);
+    if (vecs <= 8192) return launch_rows_vpt<DT, MODE, I8, V, 8, 4096, 8192>(p, di, vecs, s);
   } else {
-    if (V > 1 && vecs <= 4 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 4>(p, di, vecs, s);
-    if (V < 4 && vecs <= 8 * 1024) return launch_rows_vpt<DT, MODE, I8, V, 8>(p, di, vecs, s);
+    if (vecs <= 8192) return launch_rows_vpt<DT, MODE, I8, V, 8, 0, 8192>(p, di, vecs, s);
   }
   return launch_gemm_kernel(sp24::rows_quant_long_kernel<DT, MODE, I8>,
                             static_cast<unsigned>(p.rows), 1024, 0, s, 0, true, p);
