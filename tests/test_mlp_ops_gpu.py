@@ -764,3 +764,19 @@ def test_norm_whose_squares_are_subnormal(cols):
     eps = 2.0 ** -125
     q, s = sp24.rmsnorm_quant(x, w, eps=eps)
     check_rows(q, s, rmsnorm64(x, w, None, eps)[1], sp24.I8, scale_tol(cols))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,h,f", [(1, 8, 8), (1, 4096, 640), (5, 136, 96), (16, 1000, 264), (33, 64, 2744), (64, 1024, 256),
+                                   (100, 264, 1032), (128, 256, 256), (40, 264, 14336), (128, 72, 15000)])
+def test_ffn_few_tokens_repeat_exactly(t, h, f, dtype):
+    """Up to 128 tokens too, a call gives the same bits every time, with g and u
+    saved or not: neither the kernel nor its split of K depends on that."""
+    x, wg, wu, _ = ffn_inputs(t, h, f, dtype, seed=t)
+    want, saved = sp24.ffn_gated(x, wg, wu, save=True)
+    for _ in range(3):
+        out, again = sp24.ffn_gated(x, wg, wu, save=True)
+        assert torch.equal(out, want) and torch.equal(sp24.ffn_gated(x, wg, wu), want)
+        # rows of f sums, padded to 64: the padding is not written
+        planes, first = (s.view(torch.float32).view(2, t, -1)[:, :, :f] for s in (again, saved))
+        assert torch.equal(planes, first)
