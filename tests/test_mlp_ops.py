@@ -334,3 +334,35 @@ def test_strided_images_and_saved_buffers_are_read_as_they_are_indexed(monkeypat
     # an image that was copied is in-flight work: the launch goes without the hint
     hints = sp24.HINT_STATIC_WEIGHTS if form == "plain" else sp24.HINT_NONE
     assert seen == [(bytes(image.tolist()), hints), (bytes(saved.tolist()), None)]
+
+
+def test_type_and_shape_refusals_by_their_own_message():
+    """The checks that follow the one for a GPU, reached without it."""
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    x8, image = torch.zeros(4, 128, dtype=torch.int8), torch.zeros(4096, dtype=torch.uint8)
+    a_c = torch.zeros(128, 64, dtype=torch.int8)
+
+    def rows(x, qdtype=sp24.I8, up=None, weight=None, residual=None):
+        return sp24._rows_quant(0, "sp24_rows", x, qdtype, up, weight, residual, 0.0)
+
+    for message, call in (
+            ("qdtype 5", lambda: rows(x, sp24.E5M2)),
+            ("float16 or bfloat16 rows, not torch.float32", lambda: rows(x.float())),
+            ("torch.float16 beside torch.bfloat16", lambda: rows(x, up=x.half())),
+            ("x: a 2-D tensor", lambda: rows(x[0])),
+            ("up: shape", lambda: rows(x, up=x[:, :32])),
+            ("weight: shape", lambda: rows(x, weight=x[0, :32])),
+            ("residual: shape", lambda: rows(x, residual=x[:2])),
+            ("tokens and", lambda: sp24._gemm_scaled(0, a_c.float(), image, x8, None, None, None, None)),
+            ("out_dtype", lambda: sp24._gemm_scaled(0, a_c, image, x8, None, None, None, torch.int8)),
+            ("meta_tc: 4080 bytes", lambda: sp24._gemm_scaled(0, a_c, image[16:], x8, None, None, None, None)),
+            ("scale_w: 128", lambda: sp24._gemm_scaled(0, a_c, image, x8, torch.ones(4), None, None, None)),
+            ("scale_x: 4", lambda: sp24._gemm_scaled(0, a_c, image, x8, None, torch.ones(4).double(), None, None)),
+            ("one of float16 and", lambda: sp24._ffn_args(x, x.half(), x, sp24.ACT_SILU)),
+            ("w_up: shape", lambda: sp24._ffn_args(x, x, x[:2], sp24.ACT_SILU)),
+            ("torch.float16 beside", lambda: sp24._ffn_backward(0, x.half(), x, x, x, image, 1, True, True)),
+            ("d_out: shape", lambda: sp24._ffn_backward(0, x, x, x, x, image, 1, True, True))):
+        with pytest.raises(ValueError, match=message):
+            call()
+    with pytest.raises(ValueError, match="CUDA tensors are wanted"):
+        sp24.quantize_rows(x)
