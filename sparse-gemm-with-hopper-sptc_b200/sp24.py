@@ -420,14 +420,11 @@ def _tma_rows(t, what, cols=None, rows=None):
     return padded, ld
 
 
-def _fresh_copies(lib, copied, call, *args):
-    """call(*args).  `copied`: a weight operand was copied on the stream just
-    now, so whatever the caller says of its own weights, this launch may not
-    load them before the work ahead of it is done.  The hint is the calling
-    thread's own."""
-    hints = lib.sp24_get_launch_hints() if copied else 0
-    if not hints & HINT_STATIC_WEIGHTS:
-        return call(*args)
+def _after_copies(lib, call, *args):
+    """call(*args) where a weight operand was copied on the stream just now:
+    whatever the caller says of its own weights, this launch may not load them
+    before the work ahead of it is done.  The hint is the calling thread's own."""
+    hints = lib.sp24_get_launch_hints()
     lib.sp24_set_launch_hints(hints & ~HINT_STATIC_WEIGHTS)
     try:
         return call(*args)
@@ -560,7 +557,7 @@ def _gemm_scaled(s, a_c, meta_tc, x, scale_w, scale_x, bias, out_dtype):
                          "both float8_e4m3fn are wanted")
     if out is None:
         raise ValueError(f"gemm_scaled: out_dtype {out_dtype}")
-    given = a_c, meta_tc
+    given, copied = a_c, False
     a_c, lda = _tma_rows(a_c, "a_c")
     m, k = a_c.shape[0], 2 * a_c.shape[1]
     x, ldx = _tma_rows(x, "x", k)
@@ -569,15 +566,18 @@ def _gemm_scaled(s, a_c, meta_tc, x, scale_w, scale_x, bias, out_dtype):
     if meta_tc.nbytes != image:
         raise ValueError(f"meta_tc: {meta_tc.nbytes} bytes, {image} expected")
     if not meta_tc.is_contiguous():
-        meta_tc = meta_tc.contiguous()
+        meta_tc, copied = meta_tc.contiguous(), True
     scale_w, p_w = _vector_f32(scale_w, m, "scale_w")
     scale_x, p_x = _vector_f32(scale_x, n, "scale_x")
     bias, p_b = _vector_f32(bias, m, "bias")
     c = x.new_empty((n, m), dtype=out_dtype or torch.bfloat16)
     d = _PACK_SCALED(code, out, m, n, k, a_c.data_ptr(), lda, meta_tc.data_ptr(), x.data_ptr(), ldx,
                      p_w, p_x, p_b, c.data_ptr(), 0, 0)
-    copied = a_c is not given[0] or meta_tc is not given[1]
-    _check(_fresh_copies(lib, copied, lib.sp24_gemm_scaled, d, s), "sp24_gemm_scaled")
+    if copied or a_c is not given:
+        code = _after_copies(lib, lib.sp24_gemm_scaled, d, s)
+    else:
+        code = lib.sp24_gemm_scaled(d, s)
+    _check(code, "sp24_gemm_scaled")
     return c
 
 
@@ -617,9 +617,12 @@ def _ffn_forward(s, x, w_gate, w_up, act, save):
         n_saved = lib.sp24_ffn_saved_bytes(t, f)
         saved = x.new_empty((n_saved,), dtype=torch.uint8)
         p_saved = saved.data_ptr()
-    copied = keep[1] is not w_gate or keep[2] is not w_up
-    _check(_fresh_copies(lib, copied, lib.sp24_ffn_forward, _PACK_FFN(*args, p_saved, n_saved, 0),
-                         out.data_ptr(), 0, s), "sp24_ffn_forward")
+    call = _PACK_FFN(*args, p_saved, n_saved, 0), out.data_ptr(), 0, s
+    if keep[1] is not w_gate or keep[2] is not w_up:
+        code = _after_copies(lib, lib.sp24_ffn_forward, *call)
+    else:
+        code = lib.sp24_ffn_forward(*call)
+    _check(code, "sp24_ffn_forward")
     del keep
     return (out, saved) if save else out
 
