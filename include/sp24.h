@@ -165,7 +165,8 @@ sp24_status sp24_gemm(const sp24_gemm_desc* d, sp24_stream_t stream);
 sp24_status sp24_last_kernel_status(sp24_stream_t stream);
 
 /* Launch hints for later GEMM calls made from the calling host thread (no
-   reference counterpart; sp24_gemm_scaled and sp24_ffn_forward take them too).  GEMM kernels are launched with programmatic
+   reference counterpart; sp24_gemm_scaled and sp24_ffn_forward take them
+   too).  GEMM kernels are launched with programmatic
    dependent launch: they may start while the previous kernel of the stream
    finishes and wait for it before their first load.
    SP24_HINT_STATIC_WEIGHTS: the caller guarantees that A_c and the metadata
@@ -331,7 +332,8 @@ sp24_status sp24_gemm_scaled(const sp24_scaled_desc* d, sp24_stream_t stream);
      dx = dg w_gate + du w_up,  dw_gate = dg^T x,  dw_up = du^T x
    Sums are fp32.  g and u are never rounded: the forward pass hands them to
    the backward pass in fp32 through `saved`.  dg and du are rounded to dtype
-   (they are tensor-core operands); every output is rounded once.
+   (they are tensor-core operands), so in SP24_F16 they want a scaled loss: beyond
+   65504 they become infinite, below 2^-25 zero.  Every output is rounded once.
    x, w_gate and w_up rows must start on 16-byte boundaries (SP24_ERR_ALIGN);
    saved and the workspace on 32-byte ones.  out, d_out and the gradients have no alignment
    rule. */

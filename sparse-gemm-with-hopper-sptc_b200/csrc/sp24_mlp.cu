@@ -406,9 +406,10 @@ sp24_status scaled_pair(const FfnCall& c, const sp24_scaled_desc* d) {
 // two blocks x 224 tokens load less per product: a wave of the large tile takes
 // twice as long as one of the small (K = 14336: 47 and 25 us; K = 4096: 18 and 8),
 // and its last wave may go in halves.  The large tile is taken where it ends
-// sooner (4096 tokens x 4096 x 14336: 2.5 large waves or 7 small, 137 and 178 us;
-// 1024 tokens x 14336 x 4096: 2 or 7, 40.6 and 53.4 us; 333 x 5003 x 4160: half a
-// wave or one, 16.3 and 12.4 us, and a tie goes to the small).
+// sooner.  Device times of both in a burst / held under the power cap: 4096 tokens x
+// 4096 x 14336, 2.5 large waves or 7 small, 125 / 140 and 160 / 180 us; 1024 tokens x
+// 14336 x 4096, 2 or 7, 41 / 45 and 54 / 56 us; 333 x 5003 x 4160, half a wave or
+// one, 18.7 / 18.4 and 14.0 / 13.8 us, and a tie goes to the small.
 template <int I8>
 sp24_status scaled(const FfnCall& c, const sp24_scaled_desc* d) {
   const long long pairs = c.sm_count / 2;

@@ -18,11 +18,11 @@
 //   MB = 1, BN = 128  36 KB per 360 clocks: more loading per product, but twice
 //                     as many tiles in both directions and two accumulator
 //                     buffers, for calls that do not fill the GPU with the other.
-// 14336 x 4096 int8, 4096 tokens (481 dense-equivalent GFLOP): 134 us in a burst,
-// 145 held under the 1000 W cap at 1.69 GHz, where the MMAs alone would take 86.
-// Filling the stages and feeding the MMAs slow each other: without its stores the
-// kernel takes 115 us, without its MMAs 114, without its loads 117.  Measured and
-// not kept: 128-byte store lines (144 against 144), cache policies on weights or
+// 14336 x 4096 int8, 4096 tokens (481 dense-equivalent GFLOP): 130-134 us in a
+// burst, 145-148 held under the 1000 W cap at 1.69 GHz, where the MMAs alone would
+// take 86.  Filling the stages and feeding the MMAs slow each other: without its
+// stores the kernel takes 115 us, without its MMAs 114, without its loads 117.
+// Measured and not kept (times held under the cap): 128-byte store lines (144 against 144), cache policies on weights or
 // output (the same), both accumulators packed before the first store (164),
 // starting block 0 while block 1 drains (148; with three stages ahead 147), three
 // accumulators of 160 columns, so that every epilogue overlaps (155 against 141),

@@ -630,7 +630,8 @@ def _ffn_forward(s, x, w_gate, w_up, act, save):
 def ffn_gated(x, w_gate, w_up, *, act=ACT_SILU, save=False, stream=None):
     """sp24_ffn_forward: act(x w_gate^T) * (x w_up^T) -> [t, f], act one of
     ACT_SILU, ACT_GELU_TANH and ACT_NONE; with save=True also the opaque buffer
-    that ffn_gated_backward takes."""
+    that ffn_gated_backward takes.  No autograd graph is recorded, not for inputs
+    that require gradients either: they come from ffn_gated_backward."""
     return _on(_same_device(x, w_gate, w_up), stream, _ffn_forward, x, w_gate, w_up, act, save)
 
 
